@@ -182,6 +182,44 @@ CacheView view_of(const FridayKV* kv) {
     return v;
 }
 
+StepContext context_of(const FridayGeometry* g) {
+    StepContext ctx;
+    ctx.rows = g->rows;
+    ctx.n_seqs = g->n_seqs;
+    ctx.max_q_len = g->max_q_len;
+    ctx.max_kv_len = g->max_kv_len;
+    ctx.decode = g->decode != 0;
+    ctx.row_seq = g->row_seq;
+    ctx.row_pos = g->row_pos;
+    ctx.seq_start = g->seq_start;
+    ctx.seq_qlen = g->seq_qlen;
+    ctx.seq_pos0 = g->seq_pos0;
+    return ctx;
+}
+
+// The handle's device for the length of a call; the thread's own afterwards.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        cuda_check(cudaGetDevice(&before), "cudaGetDevice");
+        if (before == device) before = -1;
+        else cuda_check(cudaSetDevice(device), "cudaSetDevice");
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+Ops::AxesSpec axes_of(const int* sections, int axes, int interleaved, int neighbours, const float* denominators) {
+    if (!sections || axes < 1 || axes > 4) throw KernelError(format("1 to 4 sections are wanted, got %d", axes));
+    Ops::AxesSpec s;
+    s.sections.assign(sections, sections + axes);
+    s.interleaved = interleaved != 0;
+    s.neighbours = neighbours != 0;
+    s.denominators = denominators;
+    return s;
+}
+
 struct OpsHandle {
     std::unique_ptr<Ops> ops;
     std::unique_ptr<Arena> arena;
@@ -751,18 +789,46 @@ FR_API int friday_ops_linear_swiglu(void* h, const FridayTensor* x, const Friday
 FR_API int friday_ops_attention(void* h, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
                                 const FridayGeometry* g, int nq, int nkv, int hd, int window, float scale) {
     GUARD({
-        StepContext ctx;
-        ctx.rows = g->rows;
-        ctx.n_seqs = g->n_seqs;
-        ctx.max_q_len = g->max_q_len;
-        ctx.max_kv_len = g->max_kv_len;
-        ctx.decode = g->decode != 0;
-        ctx.row_seq = g->row_seq;
-        ctx.row_pos = g->row_pos;
-        ctx.seq_start = g->seq_start;
-        ctx.seq_qlen = g->seq_qlen;
-        ctx.seq_pos0 = g->seq_pos0;
+        const StepContext ctx = context_of(g);
         ((OpsHandle*)h)->begin().attention(*T(q), q_stride, *T(out), view_of(kv), ctx, nq, nkv, hd, window, scale);
+    })
+}
+FR_API int friday_ops_rotate_axes(void* h, const FridayTensor* x, FridayTensor* out, const int* positions, const float* denominators,
+                                  const int* sections, int axes, int interleaved, int neighbours, int heads, int head_dim, void* stream) {
+    GUARD({
+        Ops& ops = *((OpsHandle*)h)->ops;
+        OnDevice on(ops.device());
+        const Ops::Place place{(cudaStream_t)stream, nullptr, 0};
+        ops.rotate_axes(*T(x), *T(out), positions, axes_of(sections, axes, interleaved, neighbours, denominators), heads, head_dim, &place);
+    })
+}
+FR_API int friday_ops_rope_axes_kv_write(void* h, const FridayTensor* qkv, FridayTensor* q_out, const int* row_seq, const int* row_pos,
+                                         const int* positions, const float* denominators, const int* sections, int axes, int interleaved,
+                                         int neighbours, int nq, int nkv, int hd, const FridayKV* kv, int n_seqs, void* stream) {
+    GUARD({
+        Ops& ops = *((OpsHandle*)h)->ops;
+        OnDevice on(ops.device());
+        const Ops::Place place{(cudaStream_t)stream, nullptr, 0};
+        ops.rope_axes_kv_write(*T(qkv), q_out ? T(q_out) : nullptr, row_seq, row_pos, positions,
+                               axes_of(sections, axes, interleaved, neighbours, denominators), nq, nkv, hd, view_of(kv), n_seqs, &place);
+    })
+}
+FR_API int friday_ops_attention_shared_floats(void* h, int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int nq, int nkv,
+                                              int hd, int window, int dtype, int64_t* floats) {
+    GUARD({
+        Ops& ops = *((OpsHandle*)h)->ops;
+        OnDevice on(ops.device());
+        *floats = ops.attention_shared_floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, nq, nkv, hd, window, (DType)dtype);
+    })
+}
+FR_API int friday_ops_attention_shared(void* h, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
+                                       const int* prefix_table, int prefix_len, const FridayGeometry* g, int nq, int nkv, int hd, int window,
+                                       float scale, float* scratch, int64_t scratch_floats, void* stream) {
+    GUARD({
+        Ops& ops = *((OpsHandle*)h)->ops;
+        OnDevice on(ops.device());
+        const Ops::Place place{(cudaStream_t)stream, scratch, scratch_floats};
+        ops.attention_shared(*T(q), q_stride, *T(out), view_of(kv), prefix_table, prefix_len, context_of(g), nq, nkv, hd, window, scale, &place);
     })
 }
 FR_API int friday_ops_sample(void* h, const FridayTensor* logits, const float* temperature, const int* streams,

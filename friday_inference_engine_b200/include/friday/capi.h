@@ -147,6 +147,20 @@ int friday_ops_linear_swiglu(void* ops, const FridayTensor* x, const FridayTenso
                              const FridayTensor* weight_pairs, FridayTensor* out);
 int friday_ops_attention(void* ops, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
                          const FridayGeometry* geometry, int n_heads, int n_kv_heads, int head_dim, int window, float scale);
+/* Rotary positions with several axes, their append to the cache, attention of a batch with a shared prefix (friday::Ops::rotate_axes,
+ * rope_axes_kv_write, attention_shared).  They run on the stream that is given, use nothing of the handle that another call could be
+ * using, and leave the calling thread's current device as it was.  sections: host, [axes]; out, q_out and scratch are the caller's. */
+int friday_ops_rotate_axes(void* ops, const FridayTensor* x, FridayTensor* out, const int* positions, const float* denominators,
+                           const int* sections, int axes, int interleaved, int neighbours, int heads, int head_dim, void* stream);
+int friday_ops_rope_axes_kv_write(void* ops, const FridayTensor* qkv, FridayTensor* q_out, const int* row_seq, const int* row_pos,
+                                  const int* positions, const float* denominators, const int* sections, int axes, int interleaved,
+                                  int neighbours, int n_heads, int n_kv_heads, int head_dim, const FridayKV* kv, int n_seqs, void* stream);
+/* floats of scratch that an attention_shared of these sizes needs (dtype: 0 float32, 1 bfloat16) */
+int friday_ops_attention_shared_floats(void* ops, int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int n_heads,
+                                       int n_kv_heads, int head_dim, int window, int dtype, int64_t* floats);
+int friday_ops_attention_shared(void* ops, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
+                                const int* prefix_table, int prefix_len, const FridayGeometry* geometry, int n_heads, int n_kv_heads,
+                                int head_dim, int window, float scale, float* scratch, int64_t scratch_floats, void* stream);
 int friday_ops_sample(void* ops, const FridayTensor* logits, const float* temperature, const int* streams, const int* steps,
                       uint64_t seed, const int* row_live, int* out);
 int friday_ops_plan(void* ops, int64_t rows, int64_t n, int64_t k, int* swapped, int* bn, int* splits);

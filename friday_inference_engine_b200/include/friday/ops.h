@@ -394,6 +394,48 @@ public:
     void attention(const Tensor& q, int64_t q_stride, Tensor& out, const CacheView& view, const StepContext& ctx,
                    int n_heads, int n_kv_heads, int head_dim, int window, float scale, float out_scale = 1.0f);
 
+    // ---- a batch whose sequences share a long prefix, and rotary positions with several axes (csrc/rope_axes.cu,
+    // csrc/attention_shared.cu)
+    // Where a call runs and what it works in, if not the Ops object's stream and arena: the caller's stream, and scratch that the
+    // caller keeps until the work is done.  With a Place a call touches nothing of the Ops object that another call could.
+    struct Place {
+        cudaStream_t stream = nullptr;
+        float* scratch = nullptr;
+        int64_t scratch_floats = 0;
+    };
+    // Pair i of a head turns by position[axis(i)] / denominators[i].  Sections in turn: the first sections[0] pairs belong to axis 0,
+    // the next sections[1] to axis 1, ...  Interleaved over n axes: pair i belongs to axis i mod n if i < n * sections[i mod n], else
+    // to axis 0.  Up to 4 axes; dimensions behind the sections' pairs stay.
+    struct AxesSpec {
+        std::vector<int> sections;
+        bool interleaved = false;
+        bool neighbours = false;                    // the pairs are (2i, 2i + 1) instead of (i, i + pairs)
+        const float* denominators = nullptr;        // device [sum of sections], not zero
+    };
+    // The first `heads` heads of every row of x, turned, into out [rows, heads * head_dim]; out may be x's own columns, or columns of
+    // the same rows beside them.  positions: device [rows][axes]
+    void rotate_axes(const Tensor& x, Tensor& out, const int* positions, const AxesSpec& spec, int heads, int head_dim,
+                     const Place* place = nullptr);
+    // Rows [queries | keys | values] of qkv: queries turned into q_out [rows, n_heads * head_dim] (which may be qkv's own query
+    // columns; n_heads 0: null), keys turned and values as they are into the cache rows of (row_seq, row_pos).  The place in the cache
+    // and the positions that turn are different numbers.  Rows whose row_seq is negative are left alone; a row whose place the table
+    // does not name only gets its queries.  No two rows of a call may name the same place.
+    void rope_axes_kv_write(const Tensor& qkv, Tensor* q_out, const int* row_seq, const int* row_pos, const int* positions,
+                            const AxesSpec& spec, int n_heads, int n_kv_heads, int head_dim, const CacheView& view, int n_seqs,
+                            const Place* place = nullptr);
+    // Attention of the step's rows where every sequence begins with the same prefix_len positions: those keys and values lie in the
+    // pages of prefix_table (device), a sequence's further ones in its row of the view's block table, from the first page on.  A row
+    // at position p sees position j if p - window < j <= p (window 0: every j <= p); one that sees nothing gives zeros; one whose
+    // row_seq is negative is not written.  Pages that a table leaves out read as zeros.  The rows of sequence s are ctx.seq_start[s]
+    // and the seq_qlen[s] - 1 after it; ctx.max_kv_len bounds the positions (prefix included) and only shares the work out.
+    // Prefix and own keys are read once for all rows that share them.  prefix_len is the host's: a captured call keeps it.
+    void attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const CacheView& view, const int* prefix_table, int prefix_len,
+                          const StepContext& ctx, int n_heads, int n_kv_heads, int head_dim, int window, float scale,
+                          const Place* place = nullptr);
+    // floats of scratch that such a call needs
+    int64_t attention_shared_floats(int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int n_heads, int n_kv_heads,
+                                    int head_dim, int window, DType dtype) const;
+
     // ---- attention whose heads' scores are mixed before the softmax (csrc/attention_talk.cu)
     struct TalkSpec {
         int heads = 0, kv_heads = 0, dim = 0, vdim = 0, window = 0;

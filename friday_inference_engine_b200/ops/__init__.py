@@ -4,9 +4,12 @@ the same name (ops/ops.cpp, include/friday/ops.h), which chooses and launches th
 library's own CUDA kernels; nothing is computed here, and there is no CPU path.
 
 Kernels run on the legacy default stream, which is also torch's default, so they are
-ordered with the torch operations around them.
+ordered with the torch operations around them.  (rotate_axes, rope_axes_kv_write and
+attention_shared run on torch's current stream instead, may be captured into a CUDA graph
+there, and may be called from several threads at once.)
 """
-from ctypes import byref, c_int, c_void_p
+from ctypes import byref, c_int, c_int64, c_void_p
+from functools import lru_cache
 
 from .. import native
 
@@ -50,6 +53,22 @@ def _p(t):
 
 def _ref(struct):
     return None if struct is None else byref(struct)
+
+
+@lru_cache(maxsize=64)
+def _c_ints(values):
+    return (c_int * len(values))(*values)
+
+
+def _sections(sections):
+    """(host array, number) of the sections' pairs"""
+    try:
+        s = tuple(int(n) for n in sections)
+    except (TypeError, ValueError):
+        raise native.KernelError("sections are numbers of pairs, one per axis, got %r" % (sections,)) from None
+    if not 1 <= len(s) <= 4 or min(s) < 0 or sum(s) < 1:
+        raise native.KernelError("1 to 4 sections with at least one pair between them are wanted, got %r" % (sections,))
+    return _c_ints(s), len(s), sum(s)
 
 
 class DeferredNorm:
@@ -97,6 +116,7 @@ class CudaOps:
     name = "cuda"
 
     def __init__(self, device=0):
+        self.device = int(device)
         self._h = c_void_p()
         native.call("friday_ops_new", int(device), None, byref(self._h))
 
@@ -246,6 +266,146 @@ class CudaOps:
         native.call("friday_ops_attention_splits", self._h, rows, n_heads, max_kv_len, byref(s))
         return s.value
 
+    # -- a batch that shares a long prefix, positions with several axes ----
+    # These run on torch's current stream; what a call needs of scratch is torch's, so that a captured graph has its own.
+    def _stream(self):
+        import torch
+        return torch._C._cuda_getCurrentRawStream(self.device)
+
+    def _on_device(self, what, **tensors):
+        for name, t in tensors.items():
+            if t is not None and (not t.is_cuda or t.get_device() != self.device):
+                raise native.KernelError("%s: %s is on %s, these operations are cuda:%d's" % (what, name, t.device, self.device))
+
+    def _whole_numbers(self, what, at_least, **tensors):
+        """Tensors that kernels index as plain int32 arrays."""
+        import torch
+        self._on_device(what, **tensors)
+        for name, t in tensors.items():
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise native.KernelError("%s: %s must be contiguous int32, got %s with strides %s" % (what, name, t.dtype, t.stride()))
+            if t.numel() < at_least:
+                raise native.KernelError("%s: %s has %d numbers, %d are needed" % (what, name, t.numel(), at_least))
+
+    def _axes(self, what, rows, positions, denom, sections):
+        import torch
+        array, axes, pairs = _sections(sections)
+        self._whole_numbers(what, rows * axes, positions=positions)
+        if positions.dim() != 2 or positions.shape[0] != rows or positions.shape[1] != axes:
+            raise native.KernelError("%s: positions must be [%d rows, %d axes], got %s" % (what, rows, axes, tuple(positions.shape)))
+        self._on_device(what, denom=denom)
+        if denom.dtype != torch.float32 or not denom.is_contiguous() or denom.numel() != pairs:
+            raise native.KernelError("%s: denom must be %d contiguous float32 numbers, one per pair" % (what, pairs))
+        return array, axes
+
+    def _pools(self, what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim):
+        self._on_device(what, k_pool=k_pool, v_pool=v_pool)
+        if k_pool.dtype not in _codes() or k_pool.dtype != v_pool.dtype:
+            raise native.KernelError("%s: pools of %s and %s" % (what, k_pool.dtype, v_pool.dtype))
+        for pool in (k_pool, v_pool):
+            if pool.dim() != 4 or not pool.is_contiguous() or tuple(pool.shape[1:]) != (page_size, n_kv_heads, head_dim) or pool.shape[0] < 1:
+                raise native.KernelError("%s: pools must be contiguous [pages, %d, %d, %d], got %s" % (what, page_size, n_kv_heads, head_dim, tuple(pool.shape)))
+        if k_pool.shape[0] != v_pool.shape[0] or k_pool.data_ptr() == v_pool.data_ptr():
+            raise native.KernelError("%s: keys and values need pools of their own with the same number of pages" % what)
+        self._whole_numbers(what, 0, block_table=block_table)
+        if block_table.dim() != 2:
+            raise native.KernelError("%s: the block table is [sequences, pages], got %s" % (what, tuple(block_table.shape)))
+
+    def rotate_axes(self, x, positions, denom, sections, heads, head_dim, interleaved=False, neighbours=False, out=None):
+        """The first `heads` heads of every row of x [rows, >= heads * head_dim], turned: pair i of a head by
+        positions[row][axis of i] / denom[i].  sections: pairs per axis (time, height, width; up to 4), one axis after another, or
+        with `interleaved` in turn: pair i belongs to axis i mod n if i < n * sections[i mod n], else to axis 0.  A pair is
+        (i, i + pairs), with `neighbours` (2i, 2i + 1); dimensions behind the pairs stay.  out [rows, heads * head_dim] may be x's own
+        columns (None: a new tensor).  positions int32 [rows, axes], denom float32 [pairs], not zero.  -> out"""
+        import torch
+        heads, head_dim = int(heads), int(head_dim)
+        self._on_device("rotate_axes", x=x, out=out)
+        if x.dim() != 2:
+            raise native.KernelError("rotate_axes: rows [rows, columns] are wanted, got %s" % (tuple(x.shape),))
+        array, axes = self._axes("rotate_axes", x.shape[0], positions, denom, sections)
+        if out is None:
+            out = torch.empty((x.shape[0], max(heads, 0) * max(head_dim, 0)), dtype=x.dtype, device=x.device)
+        if x.shape[0] == 0:
+            return out
+        native.call("friday_ops_rotate_axes", self._h, _t(x), _t(out), positions.data_ptr(), denom.data_ptr(), array, axes,
+                    1 if interleaved else 0, 1 if neighbours else 0, heads, head_dim, self._stream())
+        return out
+
+    def rope_axes_kv_write(self, qkv, row_seq, row_pos, positions, denom, sections, n_heads, n_kv_heads, head_dim, k_pool, v_pool,
+                           block_table, page_size, interleaved=False, neighbours=False, q_out=None):
+        """Rows [queries | keys | values] of qkv: the queries turned (see rotate_axes) into q_out [rows, n_heads * head_dim] (may be
+        qkv's own query columns; None: a new tensor), keys turned and values as they are to the cache's row of (row_seq, row_pos):
+        page block_table[row_seq][row_pos / page_size], row row_pos mod page_size.  qkv itself is left as it was.  Rows whose row_seq
+        is negative are left alone; a row whose place the table does not name only gets its queries.  No two rows of a call may name
+        the same place.  -> q_out"""
+        import torch
+        what = "rope_axes_kv_write"
+        n_heads, n_kv_heads, head_dim, page_size = int(n_heads), int(n_kv_heads), int(head_dim), int(page_size)
+        self._on_device(what, qkv=qkv, q_out=q_out)
+        if qkv.dim() != 2:
+            raise native.KernelError("%s: rows [rows, columns] are wanted, got %s" % (what, tuple(qkv.shape)))
+        rows = qkv.shape[0]
+        array, axes = self._axes(what, rows, positions, denom, sections)
+        self._whole_numbers(what, rows, row_seq=row_seq, row_pos=row_pos)
+        self._pools(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim)
+        if q_out is None:
+            q_out = torch.empty((rows, max(n_heads, 0) * head_dim), dtype=qkv.dtype, device=qkv.device)
+        if rows == 0 or block_table.shape[0] == 0:
+            return q_out
+        if block_table.shape[1] == 0:
+            raise native.KernelError("%s: the block table is empty" % what)
+        kv = _kv(k_pool, v_pool, block_table, page_size)
+        native.call("friday_ops_rope_axes_kv_write", self._h, _t(qkv), _t(q_out) if n_heads > 0 else None, row_seq.data_ptr(),
+                    row_pos.data_ptr(), positions.data_ptr(), denom.data_ptr(), array, axes, 1 if interleaved else 0,
+                    1 if neighbours else 0, n_heads, n_kv_heads, head_dim, byref(kv), block_table.shape[0], self._stream())
+        return q_out
+
+    def attention_shared(self, q, q_stride, out, k_pool, v_pool, prefix_table, prefix_len, block_table, page_size, row_seq, row_pos,
+                         n_heads, n_kv_heads, head_dim, window, scale, geometry):
+        """attention() for sequences that all begin with the same prefix_len positions.  Their keys and values lie in the pages of
+        prefix_table (int32, may be None without a prefix); block_table [sequences, pages] names each sequence's own pages, its
+        position prefix_len being the first row of the first of them.  A row at position p (row_pos, prefix included) sees position j
+        if p - window < j <= p (window 0 or None: every j <= p) and a table has room for it; a page that a table leaves out reads as
+        zeros.  A row that sees nothing gives zeros; a row whose row_seq is negative is not written.
+
+        geometry: an object with n_seqs, max_q_len, max_kv_len (prefix included) and the arrays seq_start and seq_qlen (int32,
+        device): the rows of sequence s are seq_start[s] and the seq_qlen[s] - 1 after it, row_seq says so too.  max_q_len bounds
+        seq_qlen; max_kv_len is a bound on the positions that only shares the work out.  prefix_len is a number of the host's: a
+        captured graph keeps it."""
+        import torch
+        what = "attention_shared"
+        n_heads, n_kv_heads, head_dim, page_size = int(n_heads), int(n_kv_heads), int(head_dim), int(page_size)
+        prefix_len, window, rows = int(prefix_len), int(window or 0), out.shape[0]
+        self._on_device(what, q=q, out=out)
+        self._pools(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim)
+        if q.dim() != 2 or out.dim() != 2 or (rows > 1 and q.stride(0) != q_stride):
+            raise native.KernelError("%s: rows of queries whose stride is q_stride and rows of results are wanted, got strides %s and %s, q_stride %d"
+                                     % (what, q.stride(), out.stride(), q_stride))
+        self._whole_numbers(what, rows, row_seq=row_seq, row_pos=row_pos)
+        n_seqs, max_q_len, max_kv_len = int(geometry.n_seqs), int(geometry.max_q_len), int(geometry.max_kv_len)
+        if block_table.shape[0] < n_seqs:
+            raise native.KernelError("%s: %d sequences, a block table of %d" % (what, n_seqs, block_table.shape[0]))
+        if prefix_len > 0:
+            if prefix_table is None:
+                raise native.KernelError("%s: a prefix of %d needs its pages" % (what, prefix_len))
+            self._whole_numbers(what, -(-prefix_len // page_size), prefix_table=prefix_table)
+        self._whole_numbers(what, n_seqs, seq_start=geometry.seq_start, seq_qlen=geometry.seq_qlen)
+        if rows == 0 or n_seqs <= 0:
+            return
+        floats = c_int64()
+        code = _codes()[k_pool.dtype]
+        native.call("friday_ops_attention_shared_floats", self._h, rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads,
+                    head_dim, window, code, byref(floats))
+        scratch = torch.empty((floats.value,), dtype=torch.float32, device=out.device) if floats.value else None
+        g = native.Geometry()
+        g.rows, g.n_seqs, g.max_q_len, g.max_kv_len = rows, n_seqs, max_q_len, max_kv_len
+        g.row_seq, g.row_pos = row_seq.data_ptr(), row_pos.data_ptr()
+        g.seq_start, g.seq_qlen = geometry.seq_start.data_ptr(), geometry.seq_qlen.data_ptr()
+        kv = _kv(k_pool, v_pool, block_table, page_size, write=False)
+        native.call("friday_ops_attention_shared", self._h, _t(q), int(q_stride), _t(out), byref(kv),
+                    prefix_table.data_ptr() if prefix_len > 0 else None, prefix_len, byref(g), n_heads, n_kv_heads, head_dim, window,
+                    float(scale), scratch.data_ptr() if scratch is not None else None, floats.value, self._stream())
+
     # -- one attention kernel's launcher, called directly with chosen arguments (tests of that kernel alone) -----
     def _test_buffers(self, device):
         import torch
@@ -361,6 +521,18 @@ def qkv_rope_write(*a, **k):
 
 def attention(*a, **k):
     return backend().attention(*a, **k)
+
+
+def rotate_axes(*a, **k):
+    return backend().rotate_axes(*a, **k)
+
+
+def rope_axes_kv_write(*a, **k):
+    return backend().rope_axes_kv_write(*a, **k)
+
+
+def attention_shared(*a, **k):
+    return backend().attention_shared(*a, **k)
 
 
 def sample(*a, **k):

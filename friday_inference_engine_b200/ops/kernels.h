@@ -225,6 +225,19 @@ struct AttentionTc {
     int (*extra)(const void*, int, int, void*, const void*, const void*, int, const int*, int, const int*, const int*, const int*, const int*, int,
                  int, int, int, int, int, int, float, float, const void*, int, const void*, int, int, int, int*, cudaStream_t);
 };
+struct RopeAxes {
+    last_error_fn last_error;
+    int (*rotate)(const void*, long long, void*, long long, int, int, int, const int*, int, const float*, const int*, int, int, int, cudaStream_t);
+    int (*append)(const void*, long long, void*, long long, int, int, int, int, const int*, const int*, const int*, int, const float*, const int*, int, int,
+                  void*, void*, int, int, const int*, int, int, int, cudaStream_t);
+};
+struct AttentionShared {
+    last_error_fn last_error;
+    long long (*floats)(int, int, int, int, int, int, int, int, int, int);
+    int (*launches)(int, int, int, int, int, int, int, int, int, int);
+    int (*run)(const void*, long long, void*, const void*, const void*, int, int, const int*, int, const int*, int, int, const int*, const int*, const int*,
+               const int*, int, int, int, int, int, int, int, float, float*, long long, int*, int, cudaStream_t);
+};
 struct Sampling {
     last_error_fn last_error;
     int (*sample)(const float*, int, int, int, const float*, const int*, const int*, unsigned long long, const int*, int*,
@@ -237,6 +250,8 @@ const GemmTc& gemm_tc();
 const AttentionSimt& attention_simt();
 const AttentionMma& attention_mma();
 const AttentionTc& attention_tc();
+const RopeAxes& rope_axes();
+const AttentionShared& attention_shared();
 const Sampling& sampling();
 const AttentionWindow& attention_window();
 const Residual& residual();

@@ -1716,6 +1716,122 @@ void Ops::attention(const Tensor& q, int64_t q_stride, Tensor& out, const CacheV
          "attention_simt");
 }
 
+// ------------------------------------------------------------------ a shared prefix, positions with several axes
+namespace {
+// Two sets of rows of `n` columns each: true if a number could belong to both.  The same first column and row length (in place), or
+// columns beside one another of rows of one length, are apart.
+bool rows_collide(const Tensor& a, const Tensor& b, int64_t n, bool same_is_fine) {
+    if (a.rows() <= 0 || b.rows() <= 0) return false;
+    const int64_t es = (int64_t)dtype_size(a.dtype);
+    const char *pa = (const char*)a.data, *pb = (const char*)b.data;
+    const int64_t la = ((a.rows() - 1) * a.ld + n) * es, lb = ((b.rows() - 1) * b.ld + n) * es;
+    if (pa + la <= pb || pb + lb <= pa) return false;
+    if (pa == pb && same_is_fine && (a.ld == b.ld || a.rows() == 1)) return false;
+    if (a.ld != b.ld || (pb - pa) % es) return true;
+    const int64_t step = (((pb - pa) / es) % a.ld + a.ld) % a.ld;
+    return step < n || step > a.ld - n;
+}
+
+void check_rows(const char* what, const Tensor& t, int64_t columns) {
+    if (t.ndim != 2 || (t.dtype != DType::F32 && t.dtype != DType::BF16) || t.cols() < columns || (t.rows() > 1 && t.ld < t.cols()))
+        throw KernelError(format("%s: rows of float32 or bfloat16 with at least %lld columns are wanted", what, (long long)columns));
+}
+
+void check_axes(const char* what, const Ops::AxesSpec& s, const int* positions) {
+    if (s.sections.empty() || s.sections.size() > 4) throw KernelError(format("%s: 1 to 4 sections, got %d", what, (int)s.sections.size()));
+    if (!s.denominators || !positions) throw KernelError(format("%s: denominators and positions are needed", what));
+}
+}  // namespace
+
+void Ops::rotate_axes(const Tensor& x, Tensor& out, const int* positions, const AxesSpec& spec, int heads, int head_dim, const Place* place) {
+    const int64_t n = (int64_t)heads * head_dim;
+    if (heads < 1 || head_dim < 1) throw KernelError(format("rotate_axes: %d heads of %d numbers", heads, head_dim));
+    check_rows("rotate_axes", x, n);
+    check_rows("rotate_axes", out, n);
+    check_axes("rotate_axes", spec, positions);
+    if (out.rows() != x.rows() || out.dtype != x.dtype) throw KernelError("rotate_axes: the result needs the rows and the dtype of what is turned");
+    if (x.rows() > 0x7fffffff) throw KernelError("rotate_axes: too many rows");
+    if (rows_collide(x, out, n, true)) throw KernelError("rotate_axes: the result overlaps what is turned and is not the same columns");
+    const auto& k = kernels::rope_axes();
+    std::unique_ptr<Timed> t(place ? nullptr : new Timed(*this, Other));
+    const int rc = k.rotate(x.data, x.ld, out.data, out.ld, (int)x.rows(), heads, head_dim, positions, (int)spec.sections.size(), spec.denominators,
+                            spec.sections.data(), spec.interleaved, spec.neighbours, code(x.dtype), place ? place->stream : stream_);
+    if (rc != 0) throw KernelError(std::string("rotate_axes: ") + k.last_error());
+    __atomic_add_fetch(&launches_, x.rows() > 0 ? 1 : 0, __ATOMIC_RELAXED);
+}
+
+void Ops::rope_axes_kv_write(const Tensor& qkv, Tensor* q_out, const int* row_seq, const int* row_pos, const int* positions, const AxesSpec& spec,
+                             int n_heads, int n_kv_heads, int head_dim, const CacheView& view, int n_seqs, const Place* place) {
+    if (n_heads < 0 || n_kv_heads < 1 || head_dim < 1) throw KernelError(format("rope_axes_kv_write: %d heads, %d kv heads of %d numbers", n_heads, n_kv_heads, head_dim));
+    check_rows("rope_axes_kv_write", qkv, (int64_t)(n_heads + 2 * n_kv_heads) * head_dim);
+    check_axes("rope_axes_kv_write", spec, positions);
+    if (!row_seq || !row_pos) throw KernelError("rope_axes_kv_write: row_seq and row_pos are needed");
+    if (view.kind != CacheRequest::KV || !view.k_pool || !view.v_pool || !view.block_table || !view.write || view.every > 1 ||
+        (view.v_head_dim > 0 && view.v_head_dim != head_dim))
+        throw KernelError("rope_axes_kv_write needs a writable view of keys and values of one head size");
+    if (view.dtype != qkv.dtype) throw KernelError("rope_axes_kv_write: the cache's dtype differs from the rows'");
+    if (view.n_kv_heads != n_kv_heads || view.head_dim != head_dim)
+        throw KernelError(format("rope_axes_kv_write: the cache holds %d kv heads of %d numbers, not %d of %d", view.n_kv_heads, view.head_dim, n_kv_heads, head_dim));
+    if (n_heads > 0) {
+        if (!q_out) throw KernelError("rope_axes_kv_write: a place for the turned queries is needed");
+        check_rows("rope_axes_kv_write", *q_out, (int64_t)n_heads * head_dim);
+        if (q_out->rows() != qkv.rows() || q_out->dtype != qkv.dtype) throw KernelError("rope_axes_kv_write: the queries need the rows and the dtype of qkv");
+        Tensor q = qkv;                                                    // the keys and values are read too: only the query columns may be the same
+        if (rows_collide(q, *q_out, (int64_t)(n_heads + 2 * n_kv_heads) * head_dim, false) &&
+            !(q_out->data == qkv.data && (q_out->ld == qkv.ld || qkv.rows() == 1)))
+            throw KernelError("rope_axes_kv_write: the turned queries overlap qkv and are not its query columns");
+    }
+    if (qkv.rows() > 0x7fffffff) throw KernelError("rope_axes_kv_write: too many rows");
+    const auto& k = kernels::rope_axes();
+    std::unique_ptr<Timed> t(place ? nullptr : new Timed(*this, Other));
+    const int rc = k.append(qkv.data, qkv.ld, n_heads > 0 ? q_out->data : nullptr, n_heads > 0 ? q_out->ld : 0, (int)qkv.rows(), n_heads, n_kv_heads,
+                            head_dim, row_seq, row_pos, positions, (int)spec.sections.size(), spec.denominators, spec.sections.data(),
+                            spec.interleaved, spec.neighbours, view.k_pool, view.v_pool, view.pool_pages, view.page_size, view.block_table,
+                            n_seqs, view.table_width, code(qkv.dtype), place ? place->stream : stream_);
+    if (rc != 0) throw KernelError(std::string("rope_axes_kv_write: ") + k.last_error());
+    __atomic_add_fetch(&launches_, qkv.rows() > 0 ? 1 : 0, __ATOMIC_RELAXED);
+}
+
+int64_t Ops::attention_shared_floats(int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int n_heads, int n_kv_heads, int head_dim,
+                                     int window, DType dtype) const {
+    return kernels::attention_shared().floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, window, code(dtype));
+}
+
+void Ops::attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const CacheView& view, const int* prefix_table, int prefix_len,
+                           const StepContext& ctx, int n_heads, int n_kv_heads, int head_dim, int window, float scale, const Place* place) {
+    if (view.kind != CacheRequest::KV || !view.k_pool || !view.v_pool) throw KernelError("attention_shared needs a view of keys and values");
+    if (view.every > 1 || view.chunk > 0 || view.keep_first > 0 || (view.v_head_dim > 0 && view.v_head_dim != head_dim))
+        throw KernelError("attention_shared: values of the keys' head size, one row per position, no first keys kept behind a window, no runs");
+    const int64_t n = (int64_t)n_heads * head_dim;
+    if (n_heads < 1 || n_kv_heads < 1 || head_dim < 1 || n_heads % n_kv_heads) throw KernelError(format("attention_shared: %d heads on %d kv heads of %d numbers", n_heads, n_kv_heads, head_dim));
+    check_rows("attention_shared", q, n);
+    check_rows("attention_shared", out, n);
+    if (out.cols() != n || (out.rows() > 1 && !out.contiguous())) throw KernelError("attention_shared: the result is contiguous rows of heads * head_dim");
+    if (q.dtype != out.dtype || view.dtype != out.dtype) throw KernelError("attention_shared: queries, result and cache are of one dtype");
+    if (q.rows() < out.rows() || (out.rows() > 1 && q_stride != q.ld)) throw KernelError("attention_shared: the queries' rows do not match the result's");
+    if (view.n_kv_heads != n_kv_heads || view.head_dim != head_dim)
+        throw KernelError(format("attention_shared: the cache holds %d kv heads of %d numbers, not %d of %d", view.n_kv_heads, view.head_dim, n_kv_heads, head_dim));
+    if (prefix_len < 0 || (prefix_len > 0 && !prefix_table)) throw KernelError("attention_shared: a prefix needs its length and its pages");
+    const int rows = (int)out.rows();
+    if (rows <= 0) return;
+    if (ctx.n_seqs < 1 || ctx.max_q_len < 1 || !ctx.row_seq || !ctx.row_pos || !ctx.seq_start || !ctx.seq_qlen || (view.table_width > 0 && !view.block_table))
+        throw KernelError("attention_shared: the step's geometry (rows' sequences and positions, the sequences' rows) is needed");
+    Tensor q_rows = q;
+    q_rows.shape[0] = rows;
+    if (rows_collide(q_rows, out, n, false)) throw KernelError("attention_shared: the result overlaps the queries");
+    const auto& k = kernels::attention_shared();
+    const int64_t floats = attention_shared_floats(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, window, out.dtype);
+    if (place && place->scratch_floats < floats) throw KernelError(format("attention_shared: %lld floats of scratch are needed", (long long)floats));
+    float* scratch = floats == 0 ? nullptr : place ? place->scratch : scratch_floats(floats);
+    std::unique_ptr<Timed> t(place ? nullptr : new Timed(*this, Attention));
+    const int rc = k.run(q.data, q_stride, out.data, view.k_pool, view.v_pool, view.pool_pages, view.page_size, prefix_table, prefix_len, view.block_table,
+                         ctx.n_seqs, view.table_width, ctx.row_seq, ctx.row_pos, ctx.seq_start, ctx.seq_qlen, rows, ctx.max_q_len, ctx.max_kv_len, n_heads,
+                         n_kv_heads, head_dim, window, scale, scratch, floats, (int*)status_.get(), code(out.dtype), place ? place->stream : stream_);
+    if (rc != 0) throw KernelError(std::string("attention_shared: ") + k.last_error());
+    __atomic_add_fetch(&launches_, k.launches(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, window, code(out.dtype)),
+                       __ATOMIC_RELAXED);
+}
+
 // ------------------------------------------------------------------ sampling
 void Ops::sample(const Tensor& logits, const float* temperature, const int* streams, const int* steps,
                  unsigned long long seed, const int* row_live, int* out) {
