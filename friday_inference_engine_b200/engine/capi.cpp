@@ -814,11 +814,11 @@ FR_API int friday_ops_rope_axes_kv_write(void* h, const FridayTensor* qkv, Frida
     })
 }
 FR_API int friday_ops_attention_shared_floats(void* h, int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int nq, int nkv,
-                                              int hd, int window, int dtype, int64_t* floats) {
+                                              int hd, int page, int window, int dtype, int64_t* floats) {
     GUARD({
         Ops& ops = *((OpsHandle*)h)->ops;
         OnDevice on(ops.device());
-        *floats = ops.attention_shared_floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, nq, nkv, hd, window, (DType)dtype);
+        *floats = ops.attention_shared_floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, nq, nkv, hd, page, window, (DType)dtype);
     })
 }
 FR_API int friday_ops_attention_shared(void* h, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,

@@ -157,7 +157,7 @@ int friday_ops_rope_axes_kv_write(void* ops, const FridayTensor* qkv, FridayTens
                                   int neighbours, int n_heads, int n_kv_heads, int head_dim, const FridayKV* kv, int n_seqs, void* stream);
 /* floats of scratch that an attention_shared of these sizes needs (dtype: 0 float32, 1 bfloat16) */
 int friday_ops_attention_shared_floats(void* ops, int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int n_heads,
-                                       int n_kv_heads, int head_dim, int window, int dtype, int64_t* floats);
+                                       int n_kv_heads, int head_dim, int page_size, int window, int dtype, int64_t* floats);
 int friday_ops_attention_shared(void* ops, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
                                 const int* prefix_table, int prefix_len, const FridayGeometry* geometry, int n_heads, int n_kv_heads,
                                 int head_dim, int window, float scale, float* scratch, int64_t scratch_floats, void* stream);

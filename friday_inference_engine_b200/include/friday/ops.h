@@ -434,7 +434,7 @@ public:
                           const Place* place = nullptr);
     // floats of scratch that such a call needs
     int64_t attention_shared_floats(int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int n_heads, int n_kv_heads,
-                                    int head_dim, int window, DType dtype) const;
+                                    int head_dim, int page_size, int window, DType dtype) const;
 
     // ---- attention whose heads' scores are mixed before the softmax (csrc/attention_talk.cu)
     struct TalkSpec {

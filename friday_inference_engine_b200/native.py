@@ -154,7 +154,7 @@ _SIGNATURES = {
     "friday_ops_attention": [P, T, c_int64, T, POINTER(KV), POINTER(Geometry), I, I, I, I, F],
     "friday_ops_rotate_axes": [P, T, T, P, P, PI, I, I, I, I, I, P],
     "friday_ops_rope_axes_kv_write": [P, T, T, P, P, P, P, PI, I, I, I, I, I, I, POINTER(KV), I, P],
-    "friday_ops_attention_shared_floats": [P, I, I, I, I, I, I, I, I, I, I, POINTER(c_int64)],
+    "friday_ops_attention_shared_floats": [P, I, I, I, I, I, I, I, I, I, I, I, POINTER(c_int64)],
     "friday_ops_attention_shared": [P, T, c_int64, T, POINTER(KV), P, I, POINTER(Geometry), I, I, I, I, F, P, c_int64, P],
     "friday_ops_sample": [P, T, P, P, P, c_uint64, P, P],
     "friday_ops_plan": [P, c_int64, c_int64, c_int64, PI, PI, PI],

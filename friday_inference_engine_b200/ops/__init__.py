@@ -395,7 +395,7 @@ class CudaOps:
         floats = c_int64()
         code = _codes()[k_pool.dtype]
         native.call("friday_ops_attention_shared_floats", self._h, rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads,
-                    head_dim, window, code, byref(floats))
+                    head_dim, page_size, window, code, byref(floats))
         scratch = torch.empty((floats.value,), dtype=torch.float32, device=out.device) if floats.value else None
         g = native.Geometry()
         g.rows, g.n_seqs, g.max_q_len, g.max_kv_len = rows, n_seqs, max_q_len, max_kv_len

@@ -160,7 +160,7 @@ FAMILY(AttentionTc, attention_tc, "attention_tc", resolve(h, fam, "attention_tc"
        resolve(h, fam, "attention_tc_extra", t.extra);)
 FAMILY(RopeAxes, rope_axes, "rope_axes", resolve(h, fam, "rope_axes_rotate", t.rotate); resolve(h, fam, "rope_axes_append", t.append);)
 FAMILY(AttentionShared, attention_shared, "attention_shared", resolve(h, fam, "attention_shared_floats", t.floats);
-       resolve(h, fam, "attention_shared_launches", t.launches); resolve(h, fam, "attention_shared", t.run);)
+       resolve(h, fam, "attention_shared", t.run);)
 FAMILY(Sampling, sampling, "sampling", resolve(h, fam, "sampling_sample", t.sample);)
 
 }  // namespace kernels

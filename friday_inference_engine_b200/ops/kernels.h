@@ -233,10 +233,9 @@ struct RopeAxes {
 };
 struct AttentionShared {
     last_error_fn last_error;
-    long long (*floats)(int, int, int, int, int, int, int, int, int, int);
-    int (*launches)(int, int, int, int, int, int, int, int, int, int);
+    long long (*floats)(int, int, int, int, int, int, int, int, int, int, int);
     int (*run)(const void*, long long, void*, const void*, const void*, int, int, const int*, int, const int*, int, int, const int*, const int*, const int*,
-               const int*, int, int, int, int, int, int, int, float, float*, long long, int*, int, cudaStream_t);
+               const int*, int, int, int, int, int, int, int, float, float*, long long, int*, int, int*, cudaStream_t);
 };
 struct Sampling {
     last_error_fn last_error;

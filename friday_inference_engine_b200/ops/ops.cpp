@@ -1793,8 +1793,8 @@ void Ops::rope_axes_kv_write(const Tensor& qkv, Tensor* q_out, const int* row_se
 }
 
 int64_t Ops::attention_shared_floats(int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int n_heads, int n_kv_heads, int head_dim,
-                                     int window, DType dtype) const {
-    return kernels::attention_shared().floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, window, code(dtype));
+                                     int page_size, int window, DType dtype) const {
+    return kernels::attention_shared().floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, page_size, window, code(dtype));
 }
 
 void Ops::attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const CacheView& view, const int* prefix_table, int prefix_len,
@@ -1820,16 +1820,16 @@ void Ops::attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const
     q_rows.shape[0] = rows;
     if (rows_collide(q_rows, out, n, false)) throw KernelError("attention_shared: the result overlaps the queries");
     const auto& k = kernels::attention_shared();
-    const int64_t floats = attention_shared_floats(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, window, out.dtype);
+    const int64_t floats = attention_shared_floats(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, view.page_size, window, out.dtype);
     if (place && place->scratch_floats < floats) throw KernelError(format("attention_shared: %lld floats of scratch are needed", (long long)floats));
     float* scratch = floats == 0 ? nullptr : place ? place->scratch : scratch_floats(floats);
     std::unique_ptr<Timed> t(place ? nullptr : new Timed(*this, Attention));
+    int launches = 0;
     const int rc = k.run(q.data, q_stride, out.data, view.k_pool, view.v_pool, view.pool_pages, view.page_size, prefix_table, prefix_len, view.block_table,
                          ctx.n_seqs, view.table_width, ctx.row_seq, ctx.row_pos, ctx.seq_start, ctx.seq_qlen, rows, ctx.max_q_len, ctx.max_kv_len, n_heads,
-                         n_kv_heads, head_dim, window, scale, scratch, floats, (int*)status_.get(), code(out.dtype), place ? place->stream : stream_);
+                         n_kv_heads, head_dim, window, scale, scratch, floats, (int*)status_.get(), code(out.dtype), &launches, place ? place->stream : stream_);
     if (rc != 0) throw KernelError(std::string("attention_shared: ") + k.last_error());
-    __atomic_add_fetch(&launches_, k.launches(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, window, code(out.dtype)),
-                       __ATOMIC_RELAXED);
+    __atomic_add_fetch(&launches_, launches, __ATOMIC_RELAXED);
 }
 
 // ------------------------------------------------------------------ sampling
