@@ -128,79 +128,112 @@ __global__ void __launch_bounds__(128) rows_kernel(const SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ joining the parts
-// A warp per (row, head).  A part that saw no key has l = 0 and drops out; its o is not read.
-template <typename T>
-__global__ void __launch_bounds__(128) merge_kernel(const SharedArgs p) {
+// A block per (row, head): as many parts at a time as its threads make of a head's pieces (of VEC numbers), the first four of each
+// thread fetched beside the statistics.  A part that saw no key has l = 0 and drops out; what its o holds does not count.  (One warp
+// that took part after part waited for memory once for each: 16 rows x 28 heads x 75 parts of 128 in 45 us.)
+template <typename T, int VEC>
+__global__ void __launch_bounds__(VEC == 4 ? 128 : 256) merge_kernel(const SharedArgs p) {
+    constexpr int THREADS = VEC == 4 ? 128 : 256, AHEAD = 4;
+    __shared__ float weight[MOST_PARTS];
+    __shared__ float inv_sum;
+    __shared__ float partial[THREADS * VEC];
     fr_pdl_wait();
     fr_pdl_launch();
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= (long long)p.rows * p.nq) return;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const long long item = blockIdx.x;
     const int row = (int)(item / p.nq);
+    const int pieces = p.hd / VEC, at_once = THREADS / pieces, piece = tid % pieces, sub = tid / pieces;
+    const bool busy = sub < at_once;
+    const float* from = p.part + (size_t)item * p.parts * p.hd + piece * VEC;
+    float v[AHEAD][VEC];
+    auto fetch = [&](int s, float (&to)[VEC]) {
+        if (busy && s < p.parts) {
+            if (VEC == 4) *(float4*)to = *(const float4*)(from + (size_t)s * p.hd);
+            else to[0] = from[(size_t)s * p.hd];
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(sub + i * at_once, v[i]);
     const int seq = p.row_seq[row];
     if (seq < 0 || seq >= p.n_seqs) return;
-    // own parts are there for rows that the sequence's range names
-    int parts = p.parts;
-    if (p.prefix_splits > 0) {
-        const int t = row - p.seq_start[seq];
-        if (t < 0 || t >= min(p.seq_qlen[seq], p.covered)) parts = p.prefix_splits;
+    if (tid < 32) {
+        // own parts are there for rows that the sequence's range names
+        int parts = p.parts;
+        if (p.prefix_splits > 0) {
+            const int t = row - p.seq_start[seq];
+            if (t < 0 || t >= min(p.seq_qlen[seq], p.covered)) parts = p.prefix_splits;
+        }
+        // lane s has the statistics of parts s and s + 32
+        const float* stat = p.stat + 2 * (size_t)item * p.parts;
+        float m[2], l[2], f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool there = lane + 32 * i < parts;
+            const float2 ml = there ? *(const float2*)(stat + 2 * (lane + 32 * i)) : make_float2(-INFINITY, 0.f);
+            l[i] = ml.y;
+            m[i] = l[i] == 0.f ? -INFINITY : ml.x;
+        }
+        const float big = fr_warp_max(fmaxf(m[0], m[1]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f[i] = l[i] == 0.f ? 0.f : exp2f(m[i] - big);
+            weight[lane + 32 * i] = f[i];
+        }
+        const float sum = fr_warp_sum(f[0] * l[0] + f[1] * l[1]);
+        if (lane == 0) inv_sum = sum > 0.f ? 1.f / sum : sum;        // (0: nothing seen; a NaN stays one)
     }
-    // lane s has the statistics of parts s and s + 32
-    const float* stat = p.stat + 2 * (size_t)item * p.parts;
-    float m[2], l[2];
+    __syncthreads();
+    float acc[VEC];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const bool there = lane + 32 * i < parts;
-        m[i] = there ? stat[2 * (lane + 32 * i)] : -INFINITY;
-        l[i] = there ? stat[2 * (lane + 32 * i) + 1] : 0.f;
-        if (l[i] == 0.f) m[i] = -INFINITY;
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    for (int s0 = sub; s0 < p.parts; s0 += AHEAD * at_once) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int s = s0 + i * at_once;
+            const float w = busy && s < p.parts ? weight[s] : 0.f;
+            if (w != 0.f)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] = fmaf(w, v[i][j], acc[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fetch(s0 + (AHEAD + i) * at_once, v[i]);
     }
-    const float big = fr_warp_max(fmaxf(m[0], m[1]));
-    float f[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) f[i] = l[i] == 0.f ? 0.f : exp2f(m[i] - big);
-    const float sum = fr_warp_sum(f[0] * l[0] + f[1] * l[1]);
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    float acc[MOST_HEAD / 32];
-#pragma unroll
-    for (int i = 0; i < MOST_HEAD / 32; ++i) acc[i] = 0.f;
-    for (int s = 0; s < parts; ++s) {
-        const float w = __shfl_sync(0xffffffffu, s < 32 ? f[0] : f[1], s & 31);
-        if (w == 0.f) continue;
-        const float* o = p.part + ((size_t)item * p.parts + s) * p.hd;
-#pragma unroll
-        for (int i = 0; i < MOST_HEAD / 32; ++i)
-            if (lane + 32 * i < p.hd) acc[i] = fmaf(w, o[lane + 32 * i], acc[i]);
+    for (int j = 0; j < VEC; ++j) partial[tid * VEC + j] = acc[j];
+    __syncthreads();
+    // (in the order of the parts' residues, whatever the number of threads: the same bits every time)
+    for (int d = tid; d < p.hd; d += THREADS) {
+        float sum = 0.f;
+        for (int i = 0; i < at_once; ++i) sum += partial[i * p.hd + d];
+        fr_store((T*)p.out + (size_t)item * p.hd + d, sum * inv_sum);
     }
-    T* out = (T*)p.out + (size_t)item * p.hd;
-#pragma unroll
-    for (int i = 0; i < MOST_HEAD / 32; ++i)
-        if (lane + 32 * i < p.hd) fr_store(out + lane + 32 * i, acc[i] * inv);
 }
 
 // ------------------------------------------------------------------ bf16 on the tensor cores
 // Both products are tcgen05.mma with scores, weights and results in tensor memory.  A tile is 128 rows of one kv head; row r of it
 // stands for (token row r / G, group head r % G), G = heads / kv heads.  For the prefix a tile's token rows are any consecutive rows
 // of the step, whatever sequences they belong to: that is what reads the prefix once for all.  For own keys they are rows of one
-// sequence.  A CTA has TILES tiles that share the blocks of keys it walks, and one of three jobs:
+// sequence.  A CTA has one tile and one of three jobs:
 //
 //   prefix   consecutive rows of the step, a share of the prefix' blocks            -> a part
 //   own      rows of one sequence, a share of its own blocks                        -> a part
 //   whole    rows of one sequence, all of the prefix' blocks and then its own       -> the result (many rows per sequence)
 //
 //   warp 0      TMA: the queries (a 4-d box [64 dims][G heads][1][T rows] per 64-dim slice lands as rows t * G + g, 128-byte
-//               swizzle), then K of the block after and V of this one; a page that a table leaves out, or that lies behind the last
-//               key in sight, is loaded from beyond the pool's last row, which fills zeros
-//   warp 1      tensor memory; one lane issues S = Q K^T and O += P V
-//   four warps  per tile, one thread per row: maximum, exponentials, running maximum and sum; P goes back into tensor memory as bf16
-//               over its scores.  The reference maximum only moves when the true one has grown by more than 8 (in log2 units; weights
-//               stay below 2^8); O is rescaled then.
+//               swizzle), then K of the block after and V of this one (a block of 64 keys is a page); a page that a table leaves out
+//               is loaded from beyond the pool's last row, which fills zeros
+//   warp 1      tensor memory; one lane issues S = Q K^T two blocks ahead of O += P V
+//   warps 2-5   one thread per row: maximum, exponentials, running maximum and sum; P goes back into tensor memory as bf16 over its
+//               scores.  The reference maximum only moves when the true one has grown by more than 8 (in log2 units; weights stay
+//               below 2^8); O is rescaled then.
 //
-// TILES 1: blocks of 64 keys, two stages of scores, half the tensor memory, two CTAs per SM.  TILES 2: blocks of 128 keys, one stage
-// of scores per tile, the tiles take turns on the tensor core.  P is rounded to bf16 for the second product (its sum is not); scores,
-// sums and results are 32-bit.  Values of positions that no row of the CTA sees may be anything: their rows are zeroed in shared
-// memory before the product.  (A position that one row sees and another does not must hold finite values: zero times infinity.)
-// Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their loops.
+// A CTA takes 97 KB of shared memory and half the tensor memory, so two share an SM and one's softmax runs beside the other's
+// products: 16 prompts of 2,188 rows in all behind 8,000 keys, 28 heads on 4 of 128, took 250 us this way and 288 with two tiles and
+// blocks of 128 keys in one CTA per SM; 64 one-token rows behind 16,001 keys 52 and 71.  P is rounded to bf16 for the second product
+// (its sum is not); scores, sums and results are 32-bit.  Values of positions that no row of the CTA sees may be anything: their rows
+// are zeroed in shared memory before the product.  (A position that one row sees and another does not must hold finite values: zero
+// times infinity.)  Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their
+// loops.
 namespace tcore {
 
 using namespace tc;
@@ -208,14 +241,10 @@ using namespace tc;
 constexpr int ROWS = 128, PAGE = 64;
 constexpr int SLICE = ROWS * 128;         // bytes of 128 rows of 64 numbers
 
-template <int TILES>
-struct Shape {
-    static constexpr int KEYS = TILES == 2 ? 128 : 64, PAGES = KEYS / PAGE, THREADS = 64 + 128 * TILES;
-    static constexpr int KSLICE = KEYS * 128, STAGE = 2 * KSLICE;              // a block's keys (or values): two slices of 64 dims
-    static constexpr int TMEM = TILES == 2 ? 512 : 256;
-    static constexpr int SMEM = 2 * TILES * SLICE + 4 * STAGE + 1024 + 256;
-    // columns: TILES 2: tile x has S at 256 x (P over its first half) and O behind it; TILES 1: S of even blocks, S of odd blocks, O
-};
+constexpr int KEYS = 64, THREADS = 192;
+constexpr int KSLICE = KEYS * 128, STAGE = 2 * KSLICE;        // a block's keys (or values): two slices of 64 dims
+constexpr int TMEM = 256;                                     // columns: S of even blocks, S of odd blocks (P over each one's first half), O
+constexpr int SMEM = 2 * SLICE + 4 * STAGE + 1024 + 256;
 
 __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -295,21 +324,18 @@ struct Range {
     int lo, hi, first, n;
 };
 
-template <int TILES>
-__global__ void __launch_bounds__(Shape<TILES>::THREADS, TILES == 2 ? 1 : 2)
+__global__ void __launch_bounds__(THREADS, 2)
 tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
              const SharedArgs p) {
-    typedef Shape<TILES> S;
-    constexpr int KEYS = S::KEYS, KSLICE = S::KSLICE, STAGE = S::STAGE;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t* s_q = smem;                              // [tiles][2 slices][128 rows][128 B]
-    uint8_t* s_k = s_q + 2 * TILES * SLICE;           // [2 stages][2 slices][KEYS][128 B]
+    uint8_t* s_q = smem;                              // [2 slices][128 rows][128 B]
+    uint8_t* s_k = s_q + 2 * SLICE;                   // [2 stages][2 slices][KEYS][128 B]
     uint8_t* s_v = s_k + 2 * STAGE;
     uint64_t* bars = (uint64_t*)(s_v + 2 * STAGE);
     // bars: q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2]
     uint32_t* tmem_slot = (uint32_t*)(bars + 15);
-    int* s_pos = (int*)(tmem_slot + 1);               // [2 tiles][least, greatest position of a live row]
+    int* s_pos = (int*)(tmem_slot + 1);               // least, greatest position of a live row
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t q_full = smem_u32(bars), k_full = smem_u32(bars + 1), k_empty = smem_u32(bars + 3);
@@ -326,14 +352,14 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             mbar_init(s_full + 8 * b, 1);
             mbar_init(p_full + 8 * b, 128);
             mbar_init(pv_done + 8 * b, 1);
-            s_pos[2 * b] = 0x7fffffff;
-            s_pos[2 * b + 1] = -1;
         }
+        s_pos[0] = 0x7fffffff;
+        s_pos[1] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)S::TMEM)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)TMEM)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -348,99 +374,78 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     // same time.  CTAs start in the order of their index: the prefix' shares (the most work) first, a whole job's late rows first.
     const int G = p.nq / p.nkv, T = ROWS / G;         // token rows of a tile
     const bool prefix_job = !p.whole && (int)blockIdx.x < p.prefix_ctas;
-    int kvh, seq = 0, group, part, share, shares;     // group: which TILES tiles of the rows
-    int begin = 0, count = p.rows;                    // the rows that the tiles are taken from
+    int kvh, seq = 0, row0, n_tok, part, share, shares;
     if (prefix_job) {
         const int per = p.prefix_ctas / (p.nkv * p.prefix_splits);
-        group = blockIdx.x % per;
+        row0 = blockIdx.x % per * T;
         kvh = blockIdx.x / per % p.nkv;
         share = blockIdx.x / (per * p.nkv);
         shares = p.prefix_splits;
         part = share;
+        n_tok = min(T, p.rows - row0);
     } else {
-        const int x = blockIdx.x - (p.whole ? 0 : p.prefix_ctas), splits = p.whole ? 1 : p.own_splits;
-        const int per = (gridDim.x - (p.whole ? 0 : p.prefix_ctas)) / (p.n_seqs * p.nkv * splits);
+        const int x = blockIdx.x - p.prefix_ctas, splits = p.whole ? 1 : p.own_splits;
+        const int per = (gridDim.x - p.prefix_ctas) / (p.n_seqs * p.nkv * splits);
         seq = x % p.n_seqs;
         kvh = x / p.n_seqs % p.nkv;
         share = x / (p.n_seqs * p.nkv) % splits;
-        group = per - 1 - x / (p.n_seqs * p.nkv * splits);
         shares = splits;
         part = p.prefix_splits + share;
-        begin = p.seq_start[seq];
-        count = p.seq_qlen[seq];
-        if (begin < 0 || begin > p.rows) count = 0;
-        else count = min(count, p.rows - begin);
+        const int t0 = (per - 1 - x / (p.n_seqs * p.nkv * splits)) * T;
+        const int begin = p.seq_start[seq], count = begin < 0 || begin > p.rows ? 0 : min(p.seq_qlen[seq], p.rows - begin);
+        row0 = begin + t0;
+        n_tok = max(0, min(T, count - t0));
     }
-    int row0[TILES], n_tok[TILES];
-    bool active[TILES];
-#pragma unroll
-    for (int x = 0; x < TILES; ++x) {
-        const int t0 = (group * TILES + x) * T;
-        row0[x] = begin + t0;
-        n_tok[x] = max(0, min(T, count - t0));
-        for (int t = threadIdx.x; t < n_tok[x]; t += S::THREADS) {
-            const int of = p.row_seq[row0[x] + t];
+    // Keys [lo, hi] that the CTA's rows see between them: of the prefix, of own ones (numbered from the prefix' end).  Without a window
+    // a share of the prefix is the same whatever the rows' positions are.
+    Range seg0{0, -1, 0, 0}, seg1{0, -1, 0, 0};
+    if (prefix_job && p.window == 0) {
+        seg0.hi = p.prefix - 1;
+    } else {
+        for (int t = threadIdx.x; t < n_tok; t += THREADS) {
+            const int of = p.row_seq[row0 + t];
             if (of >= 0 && of < p.n_seqs) {
-                const int pos = position_of(p, row0[x] + t);
-                atomicMin(&s_pos[2 * x], pos);
-                atomicMax(&s_pos[2 * x + 1], pos);
+                const int pos = position_of(p, row0 + t);
+                atomicMin(&s_pos[0], pos);
+                atomicMax(&s_pos[1], pos);
             }
         }
-    }
-    __syncthreads();
-    int least = 0x7fffffff, most = -1;
-#pragma unroll
-    for (int x = 0; x < TILES; ++x) {
-        active[x] = s_pos[2 * x + 1] >= 0;
-        least = min(least, s_pos[2 * x]);
-        most = max(most, s_pos[2 * x + 1]);
-    }
-    Range seg[2];                                     // of the prefix, of own keys (numbered from the prefix' end)
-    {
+        __syncthreads();
+        const int least = s_pos[0], most = s_pos[1];
         const int lo = most < 0 ? 0 : fr_first_key(least, p.window, 0);
-        seg[0] = Range{lo, (p.whole || prefix_job) ? min(most, p.prefix - 1) : -1, 0, 0};
-        seg[1] = Range{max(0, lo - p.prefix), prefix_job ? -1 : most - p.prefix, 0, 0};
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            if (seg[g].hi < seg[g].lo) continue;
-            const int first = seg[g].lo / KEYS, n = seg[g].hi / KEYS - first + 1;
-            const int from = (int)((long long)n * share / shares), to = (int)((long long)n * (share + 1) / shares);
-            seg[g].first = first + from;
-            seg[g].n = to - from;
-        }
+        seg0.lo = lo;
+        seg1.lo = max(0, lo - p.prefix);
+        if (p.whole || prefix_job) seg0.hi = min(most, p.prefix - 1);
+        if (!prefix_job) seg1.hi = most - p.prefix;
     }
-    const int n_blocks = seg[0].n + seg[1].n;
+    auto take_share = [&](Range& g) {
+        if (g.hi < g.lo) return;
+        const int first = g.lo / KEYS, n = g.hi / KEYS - first + 1;
+        const int from = (int)((long long)n * share / shares), to = (int)((long long)n * (share + 1) / shares);
+        g.first = first + from;
+        g.n = to - from;
+    };
+    take_share(seg0);
+    take_share(seg1);
+    const int n_blocks = seg0.n + seg1.n;
     const int slices = (p.hd + 63) / 64;
-    auto first_key_of = [&](int i) { return (i < seg[0].n ? seg[0].first + i : seg[1].first + i - seg[0].n) * KEYS; };
+    auto first_key_of = [&](int i) { return (i < seg0.n ? seg0.first + i : seg1.first + i - seg0.n) * KEYS; };
+    auto last_key_of = [&](int i) { return i < seg0.n ? seg0.hi : seg1.hi; };
 
-    // Block i uses stage i & 1 of K and V, in their (i >> 1)-th use.
+    // Block i uses stage i & 1 of K, V and S, in their (i >> 1)-th use.
     if (warp == 0) {
         if (n_blocks > 0 && elect_one()) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
-            int there = 0;
-            for (int x = 0; x < TILES; ++x) there += active[x] ? 1 : 0;
-            mbar_expect_tx(q_full, (uint32_t)(there * slices * 64 * G * T * 2));
-            for (int x = 0; x < TILES; ++x)
-                if (active[x])
-                    for (int s = 0; s < slices; ++s)
-                        load_4d(smem_u32(s_q + (2 * x + s) * SLICE), &map_q, s * 64, 0, kvh, row0[x], q_full);
+            mbar_expect_tx(q_full, (uint32_t)(slices * 64 * G * T * 2));
+            for (int s = 0; s < slices; ++s) load_4d(smem_u32(s_q + s * SLICE), &map_q, s * 64, 0, kvh, row0, q_full);
             auto load = [&](int i, const CUtensorMap* map, uint8_t* ring, uint32_t full, uint32_t empty) {
                 const int b = i & 1, par = (i >> 1) & 1;
                 if (!mbar_wait(empty + 8 * b, par ^ 1, p.status, 1)) return false;
-                mbar_expect_tx(full + 8 * b, (uint32_t)(S::PAGES * slices * PAGE * 128));
-                const bool own = i >= seg[0].n;
-                const int j0 = first_key_of(i), hi = own ? seg[1].hi : seg[0].hi;
-                const int* table = own ? p.block_table + (size_t)seq * p.table_width : p.prefix_table;
-#pragma unroll
-                for (int pg = 0; pg < S::PAGES; ++pg) {
-                    const int j = j0 + pg * PAGE;
-                    int page = j <= hi ? table[j / PAGE] : -1;
-                    if (page < 0 || page >= p.pool_pages) page = p.pool_pages;          // beyond the pool: zeros
-                    for (int s = 0; s < slices; ++s)
-                        load_3d(smem_u32(ring) + (uint32_t)(b * STAGE + s * KSLICE + pg * PAGE * 128), map, s * 64, kvh, page * PAGE, full + 8 * b);
-                }
+                mbar_expect_tx(full + 8 * b, (uint32_t)(slices * KSLICE));
+                const int* table = i < seg0.n ? p.prefix_table : p.block_table + (size_t)seq * p.table_width;
+                int page = table[first_key_of(i) / PAGE];
+                if (page < 0 || page >= p.pool_pages) page = p.pool_pages;              // beyond the pool: zeros
+                for (int s = 0; s < slices; ++s)
+                    load_3d(smem_u32(ring) + (uint32_t)(b * STAGE + s * KSLICE), map, s * 64, kvh, page * PAGE, full + 8 * b);
                 return true;
             };
             bool ok = load(0, &map_k, s_k, k_full, k_empty);
@@ -457,109 +462,76 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             bool ok = mbar_wait(q_full, 0, p.status, 2);
             // (descriptors are made once and stepped: a lone thread issues all of this)
             const uint64_t dq0 = smem_desc(smem_u32(s_q)), dk0 = smem_desc(smem_u32(s_k)), dv0 = desc_mn(smem_u32(s_v), KSLICE, 1024);
-            auto scores = [&](int x, int i) {
+            auto scores = [&](int i) {
                 const int b = i & 1, par = (i >> 1) & 1;
                 if (!mbar_wait(k_full + 8 * b, par, p.status, 3)) return false;
                 tc_fence_after();
-                uint64_t da = dq0 + (uint64_t)(x * (2 * SLICE >> 4)), db = dk0 + (uint64_t)(b * (STAGE >> 4));
-                const uint32_t d = tmem + (TILES == 2 ? 256 * x : KEYS * b);
+                uint64_t da = dq0, db = dk0 + (uint64_t)(b * (STAGE >> 4));
+                const uint32_t d = tmem + KEYS * b;
                 for (int ks = 0; ks < k_steps; ++ks) {
                     tc_mma(d, da, db, idesc_qk, ks > 0 ? 1u : 0u);
                     // 32 bytes on in the 128-byte row; after four of them the next slice of 64 dims
                     da += (ks & 3) == 3 ? (uint64_t)((SLICE >> 4) - 6) : 2ull;
                     db += (ks & 3) == 3 ? (uint64_t)((KSLICE >> 4) - 6) : 2ull;
                 }
-                tc_commit(s_full + 8 * (TILES == 2 ? x : b));
+                tc_commit(s_full + 8 * b);
+                tc_commit(k_empty + 8 * b);
                 return true;
             };
-            auto second = [&](int x, int i) {
+            // The scores run two blocks ahead of the second product; the tensor core takes its instructions in order, so S of block i
+            // may overwrite P of block i - 2.
+            if (ok) ok = scores(0);
+            if (ok && n_blocks > 1) ok = scores(1);
+            for (int i = 0; i < n_blocks && ok; ++i) {
                 const int b = i & 1, par = (i >> 1) & 1;
-                if (!mbar_wait(v_full + 8 * b, par, p.status, 4)) return false;
-                // P of block i: the tile's i-th (TILES 2), or the stage's (i >> 1)-th
-                if (!mbar_wait(p_full + 8 * (TILES == 2 ? x : b), TILES == 2 ? i & 1 : par, p.status, 5)) return false;
+                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 4))) break;
+                if (!(ok = mbar_wait(p_full + 8 * b, par, p.status, 5))) break;
                 tc_fence_after();
-                const int hi = i < seg[0].n ? seg[0].hi : seg[1].hi;
-                const int steps = (min(KEYS, hi - first_key_of(i) + 1) + 15) / 16;
+                const int steps = (min(KEYS, last_key_of(i) - first_key_of(i) + 1) + 15) / 16;
                 uint64_t db = dv0 + (uint64_t)(b * (STAGE >> 4));
-                uint32_t pa = tmem + (TILES == 2 ? 256 * x : KEYS * b), keep = i > 0 ? 1u : 0u;
-                const uint32_t d = tmem + (TILES == 2 ? 256 * x + 128 : 128);
+                uint32_t pa = tmem + KEYS * b, keep = i > 0 ? 1u : 0u;
                 for (int ks = 0; ks < steps; ++ks) {
-                    mma_ta(d, pa, db, idesc_pv, keep);
+                    mma_ta(tmem + 2 * KEYS, pa, db, idesc_pv, keep);
                     keep = 1u;
                     pa += 8;                                   // 16 keys of P: 8 columns
                     db += (uint64_t)(16 * 128 >> 4);           // 16 keys of V
                 }
-                return true;
-            };
-            if (TILES == 2) {
-                for (int x = 0; x < TILES && ok; ++x)
-                    if (active[x]) ok = scores(x, 0);
-                if (ok) tc_commit(k_empty);
-                for (int i = 0; i < n_blocks && ok; ++i) {
-                    for (int x = 0; x < TILES && ok; ++x) {
-                        if (!active[x]) continue;
-                        ok = second(x, i);
-                        if (ok && i + 1 < n_blocks) ok = scores(x, i + 1);
-                    }
-                    if (!ok) break;
-                    tc_commit(v_empty + 8 * (i & 1));
-                    if (i + 1 < n_blocks) tc_commit(k_empty + 8 * ((i + 1) & 1));
-                }
-                if (ok) tc_commit(pv_done);
-            } else {
-                // the scores run two blocks ahead of the second product
-                for (int i = 0; i < 2 && i < n_blocks && ok; ++i) {
-                    ok = scores(0, i);
-                    if (ok) tc_commit(k_empty + 8 * (i & 1));
-                }
-                for (int i = 0; i < n_blocks && ok; ++i) {
-                    ok = second(0, i);
-                    if (!ok) break;
-                    tc_commit(pv_done + 8 * (i & 1));
-                    tc_commit(v_empty + 8 * (i & 1));
-                    if (i + 2 < n_blocks) {
-                        ok = scores(0, i + 2);
-                        if (ok) tc_commit(k_empty + 8 * (i & 1));
-                    }
-                }
+                tc_commit(pv_done + 8 * b);
+                tc_commit(v_empty + 8 * b);
+                if (i + 2 < n_blocks) ok = scores(i + 2);
             }
         }
     } else {
-        const int x = TILES == 2 ? (warp - 2) >> 2 : 0;
         const int quarter = warp & 3;                          // the tensor-memory lanes that this warp may touch: 32 * quarter ..
         const int r = quarter * 32 + lane, t = r / G, g = r - t * G;
-        const int row = row0[x] + t;
+        const int row = row0 + t;
         int pos = -1;
-        bool live = r < T * G && t < n_tok[x];
+        bool live = r < T * G && t < n_tok;
         if (live) {
             const int of = p.row_seq[row];
             live = of >= 0 && of < p.n_seqs;
             if (live) pos = position_of(p, row);
         }
         const int first = fr_first_key(pos, p.window, 0);
-        const bool any = __any_sync(0xffffffffu, live && pos >= 0);       // a warp without rows only keeps the barriers going
-        const int tile_least = s_pos[2 * x], tile_first_max = fr_first_key(s_pos[2 * x + 1], p.window, 0);
-        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-        const uint32_t t_o = tmem + lane_addr + (TILES == 2 ? 256 * x + 128 : 128);
+        const bool any = __any_sync(0xffffffffu, live);        // a warp without rows only keeps the barriers going
+        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16, t_o = tmem + lane_addr + 2 * KEYS;
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
-        const int mine = active[x] ? n_blocks : 0;
-        for (int i = 0; i < mine; ++i) {
+        for (int i = 0; i < n_blocks; ++i) {
             const int b = i & 1, par = (i >> 1) & 1;
-            const bool own = i >= seg[0].n;
-            const int j0 = first_key_of(i), base = own ? p.prefix : 0;
-            if (!(ok = mbar_wait(s_full + 8 * (TILES == 2 ? x : b), TILES == 2 ? i & 1 : par, p.status, 6))) break;
+            const bool own = i >= seg0.n;
+            const int j0 = first_key_of(i);
+            if (!(ok = mbar_wait(s_full + 8 * b, par, p.status, 6))) break;
             tc_fence_after();
-            const uint32_t t_s = tmem + lane_addr + (TILES == 2 ? 256 * x : KEYS * b);
+            const uint32_t t_s = tmem + lane_addr + KEYS * b;
             if (any) {
                 uint32_t raw[KEYS];
-#pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) ld32(t_s + 32 * c, &raw[32 * c]);
+                ld32(t_s, &raw[0]);
+                ld32(t_s + 32, &raw[32]);
                 tc_ld_wait();
-                // columns hi < j or j < lo are masked; the choice is the tile's
-                const int hi = own ? pos - p.prefix - j0 : min(pos, p.prefix - 1) - j0, lo = first - base - j0;
-                const bool need_mask = j0 + KEYS - 1 > (own ? tile_least - p.prefix : min(tile_least, p.prefix - 1)) || j0 < tile_first_max - base;
-                if (need_mask) {
+                // columns hi < j or j < lo are masked; most blocks need no mask for any of the warp's rows
+                const int hi = (own ? pos - p.prefix : min(pos, p.prefix - 1)) - j0, lo = first - (own ? p.prefix : 0) - j0;
+                if (__any_sync(0xffffffffu, live && (hi < KEYS - 1 || lo > 0))) {
 #pragma unroll
                     for (int j = 0; j < KEYS; ++j)
                         if (j > hi || j < lo) raw[j] = 0xff800000u;      // -inf
@@ -577,12 +549,10 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                         l_run *= alpha;
                     }
                     if (i > 0) {
-                        // Every product into O so far must be done.  TILES 2: this block's scores were issued behind them.  TILES 1:
-                        // those of block i - 2 likewise, so the wait for the other stage's phase is unambiguous.
-                        if (TILES == 1) {
-                            if (!(ok = mbar_wait(pv_done + 8 * (b ^ 1), ((i - 1) >> 1) & 1, p.status, 8))) break;
-                            tc_fence_after();
-                        }
+                        // Every product into O so far must be done: that of block i - 2 is (this block's scores were issued behind
+                        // it), so the wait for the other stage's phase is unambiguous.
+                        if (!(ok = mbar_wait(pv_done + 8 * (b ^ 1), ((i - 1) >> 1) & 1, p.status, 8))) break;
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < p.hd; c += 16) {
                             uint32_t o16[16];
@@ -598,28 +568,24 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 // a masked score is -inf and stays so; a row that has seen no key takes its exponentials against 0
                 const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
                 float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t packed[KEYS / 2];
 #pragma unroll
-                for (int h = 0; h < KEYS / 64; ++h) {
-                    uint32_t packed[32];
-#pragma unroll
-                    for (int j = 0; j < 64; j += 2) {
-                        const float e0 = exp2_fast(fmaf(__uint_as_float(raw[64 * h + j]), p.scale_log2, neg_m));
-                        const float e1 = exp2_fast(fmaf(__uint_as_float(raw[64 * h + j + 1]), p.scale_log2, neg_m));
-                        sum4[j & 2] += e0;
-                        sum4[(j & 2) + 1] += e1;
-                        packed[j >> 1] = pack2(e0, e1);
-                    }
-                    st32(t_s + 32 * h, packed);
+                for (int j = 0; j < KEYS; j += 2) {
+                    const float e0 = exp2_fast(fmaf(__uint_as_float(raw[j]), p.scale_log2, neg_m));
+                    const float e1 = exp2_fast(fmaf(__uint_as_float(raw[j + 1]), p.scale_log2, neg_m));
+                    sum4[j & 2] += e0;
+                    sum4[(j & 2) + 1] += e1;
+                    packed[j >> 1] = pack2(e0, e1);
                 }
+                st32(t_s, packed);
                 st_wait();
                 l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
             }
-            const Range& here = seg[own ? 1 : 0];
-            if (j0 < here.lo || j0 + KEYS - 1 > here.hi) {
-                // positions that no row of the CTA sees: their values may be anything (both tiles do this, each before it hands over
-                // its P of this block)
+            const int in_lo = (own ? seg1.lo : seg0.lo) - j0, in_hi = last_key_of(i) - j0;
+            if (in_lo > 0 || in_hi < KEYS - 1) {
+                // positions that no row of the CTA sees: their values may be anything
                 if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 7))) break;
-                if (r < KEYS && (j0 + r < here.lo || j0 + r > here.hi)) {
+                if (r < KEYS && (r < in_lo || r > in_hi)) {
                     for (int s = 0; s < slices; ++s) {
                         uint4* line = (uint4*)(s_v + b * STAGE + s * KSLICE + r * 128);
 #pragma unroll
@@ -629,51 +595,40 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             tc_fence_before();
-            mbar_arrive(p_full + 8 * (TILES == 2 ? x : b));
+            mbar_arrive(p_full + 8 * b);
         }
-        if (ok && mine > 0) {
-            ok = TILES == 2 ? mbar_wait(pv_done, 0, p.status, 8) : mbar_wait(pv_done + 8 * ((mine - 1) & 1), ((mine - 1) >> 1) & 1, p.status, 8);
+        if (ok && n_blocks > 0) {
+            ok = mbar_wait(pv_done + 8 * ((n_blocks - 1) & 1), ((n_blocks - 1) >> 1) & 1, p.status, 8);
             tc_fence_after();
         }
-        if (ok) {
+        if (ok && any) {
             const size_t item = (size_t)row * p.nq + (size_t)kvh * G + g;
             const bool seen = l_run != 0.f;                    // (a NaN is seen)
-            if (p.whole) {
-                const float inv = l_run > 0.f ? 1.f / l_run : l_run;
-                bf16* dst = (bf16*)p.out + item * p.hd;
+            const float inv = l_run > 0.f ? 1.f / l_run : l_run;
+            const size_t at = item * p.parts + part;
+            if (!p.whole && live) *(float2*)(p.stat + 2 * at) = make_float2(seen ? m_run : -INFINITY, l_run);
 #pragma unroll 1
-                for (int c = 0; c < p.hd; c += 16) {
-                    uint32_t o16[16];
-                    if (mine > 0) {                            // uniform: the load is warp-wide
-                        tc_ld16(t_o + c, o16);
-                        tc_ld_wait();
-                    }
-                    if (live) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            w[j] = seen ? pack2(__uint_as_float(o16[2 * j]) * inv, __uint_as_float(o16[2 * j + 1]) * inv) : 0u;
-                        *(uint4*)(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *(uint4*)(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
+            for (int c = 0; c < p.hd; c += 16) {
+                uint32_t o16[16];
+                if (n_blocks > 0) {                            // uniform: the load is warp-wide
+                    tc_ld16(t_o + c, o16);
+                    tc_ld_wait();
                 }
-            } else {
-                const size_t at = item * p.parts + part;
-                if (live) *(float2*)(p.stat + 2 * at) = make_float2(seen ? m_run : -INFINITY, l_run);
-                float* dst = p.part + at * p.hd;
-                if (mine > 0 && any) {
-#pragma unroll 1
-                    for (int c = 0; c < p.hd; c += 16) {
-                        uint32_t o16[16];
-                        tc_ld16(t_o + c, o16);
-                        tc_ld_wait();
-                        if (live && seen) {
+                if (!live) continue;
+                if (p.whole) {
+                    uint32_t w[8];
 #pragma unroll
-                            for (int j = 0; j < 16; j += 4)
-                                *(float4*)(dst + c + j) = make_float4(__uint_as_float(o16[j]), __uint_as_float(o16[j + 1]), __uint_as_float(o16[j + 2]),
-                                                                      __uint_as_float(o16[j + 3]));
-                        }
-                    }
+                    for (int j = 0; j < 8; ++j)
+                        w[j] = seen ? pack2(__uint_as_float(o16[2 * j]) * inv, __uint_as_float(o16[2 * j + 1]) * inv) : 0u;
+                    bf16* dst = (bf16*)p.out + item * p.hd + c;
+                    *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
+                    *(uint4*)(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                } else if (seen) {
+                    float* dst = p.part + at * p.hd + c;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                        *(float4*)(dst + j) = make_float4(__uint_as_float(o16[j]), __uint_as_float(o16[j + 1]), __uint_as_float(o16[j + 2]),
+                                                          __uint_as_float(o16[j + 3]));
                 }
             }
         }
@@ -682,7 +637,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)S::TMEM) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM) : "memory");
     }
 }
 
@@ -730,17 +685,20 @@ int maps(const SharedArgs& p, CUtensorMap& mq, CUtensorMap& mk, CUtensorMap& mv)
     return FR_OK;
 }
 
-template <int TILES>
-int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const SharedArgs& p, long long ctas, cudaStream_t stream) {
+int launch(const SharedArgs& p, long long ctas, cudaStream_t stream) {
+    if (ctas > 0x7fffffffLL) FR_REFUSE("attention_shared: %lld blocks exceed the grid", ctas);
+    CUtensorMap mq, mk, mv;
+    const int rc = maps(p, mq, mk, mv);
+    if (rc) return rc;
     static std::atomic<unsigned long long> configured{0};             // a bit per device
     int device = 0;
     FR_CUDA(cudaGetDevice(&device));
     const unsigned long long bit = 1ull << (device & 63);
     if (!(configured.load() & bit)) {
-        FR_CUDA(cudaFuncSetAttribute(tiles_kernel<TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<TILES>::SMEM));
+        FR_CUDA(cudaFuncSetAttribute(tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         configured.fetch_or(bit);
     }
-    FR_CUDA(fr_launch(tiles_kernel<TILES>, dim3((unsigned)ctas), dim3(Shape<TILES>::THREADS), Shape<TILES>::SMEM, stream, mq, mk, mv, p));
+    FR_CUDA(fr_launch(tiles_kernel, dim3((unsigned)ctas), dim3(THREADS), SMEM, stream, mq, mk, mv, p));
     FR_CHECK_LAUNCH("attention_shared (tiles)");
     return FR_OK;
 }
@@ -750,8 +708,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
 // ------------------------------------------------------------------ host side
 struct Plan {
     int parts = 1;
-    int tiles = 0;                                    // 0: the kernel of single rows; 1, 2: tiles per CTA of the tensor-core kernel
-    int whole = 0, prefix_splits = 0, own_splits = 0, groups = 0, own_groups = 0;      // groups of `tiles` tiles: of all rows, of a sequence's
+    int whole = 0, prefix_splits = 0, own_splits = 0, tiles = 0, own_tiles = 0;        // tiles of all rows, of a sequence's
     long long ctas = 0;
 };
 
@@ -778,30 +735,27 @@ Plan plan_tiles(long long rows, int n_seqs, int max_q_len, int max_kv_len, int p
     const int sms = fr_sm_count() > 0 ? fr_sm_count() : 148;
     const int T = tcore::ROWS / (nq / nkv);
     const long long all = (rows + T - 1) / T, own = (max_q_len + T - 1) / T;
-    int tiles = all > 1 ? 2 : 1, whole = 0, ps = -1, os = -1;
-    if (const char* e = getenv("FRIDAY_SHARED_PLAN")) sscanf(e, "%d,%d,%d,%d", &tiles, &whole, &ps, &os);
-    plan.tiles = tiles;
-    plan.groups = (int)((all + tiles - 1) / tiles);
-    plan.own_groups = (int)((own + tiles - 1) / tiles);
-    const int keys = tiles == 2 ? 128 : 64;
-    const long long slots = (long long)sms * (tiles == 2 ? 1 : 2);
+    int whole = 0, ps = -1, os = -1;
+    if (const char* e = getenv("FRIDAY_SHARED_PLAN")) sscanf(e, "%d,%d,%d", &whole, &ps, &os);
+    plan.tiles = (int)all;
+    plan.own_tiles = (int)own;
+    const long long slots = 2ll * sms, n_prefix = all * nkv, n_own = (long long)n_seqs * nkv * own;
     const long long prefix_reach = window > 0 && window < prefix ? window : prefix, own_reach = reach_of(max_kv_len - prefix, window);
-    const long long prefix_blocks = (prefix_reach + keys - 1) / keys, own_blocks = (own_reach + keys - 1) / keys;
+    const long long prefix_blocks = (prefix_reach + tcore::KEYS - 1) / tcore::KEYS, own_blocks = (own_reach + tcore::KEYS - 1) / tcore::KEYS;
     if (whole) {
         plan.whole = 1;
-        plan.ctas = (long long)n_seqs * nkv * plan.own_groups;
+        plan.ctas = n_own;
         return plan;
     }
-    const long long n_prefix = (long long)plan.groups * nkv;
     plan.prefix_splits = ps > 0 ? ps : clamp(slots / n_prefix, 1, clamp(prefix_blocks, 1, 40));
     const long long each = (prefix_blocks + plan.prefix_splits - 1) / plan.prefix_splits;
     plan.own_splits = os > 0 ? os : clamp(own_blocks / (each > 4 ? each : 4), 1, 16);
     plan.parts = plan.prefix_splits + plan.own_splits;
-    plan.ctas = n_prefix * plan.prefix_splits + (long long)n_seqs * nkv * plan.own_groups * plan.own_splits;
+    plan.ctas = n_prefix * plan.prefix_splits + n_own * plan.own_splits;
     return plan;
 }
 
-long long floats_of(const Plan& plan, long long rows, int nq, int hd) { return plan.parts > 1 ? rows * nq * plan.parts * (hd + 2) : 0; }
+long long floats_of(const Plan& plan, long long rows, int nq, int hd) { return plan.parts > 1 ? rows * nq * plan.parts * (hd + 2) + 1 : 0; }
 
 template <typename T>
 int launch_rows(const SharedArgs& p, cudaStream_t stream) {
@@ -853,15 +807,12 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     if (scratch_floats < floats_of(plan, rows, nq, hd)) FR_REFUSE("attention_shared: %lld floats of working memory are too few", scratch_floats);
     p.parts = plan.parts;
     p.part = scratch;
-    p.stat = scratch + (long long)rows * nq * plan.parts * hd;
+    p.stat = scratch + ((long long)rows * nq * plan.parts * hd + 1) / 2 * 2;           // (pairs of numbers)
     if (tiles) {
-        const int T = tcore::ROWS / (nq / nkv);
         p.whole = plan.whole; p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits;
-        p.prefix_ctas = plan.whole ? 0 : plan.groups * nkv * plan.prefix_splits;
-        p.covered = plan.own_groups * plan.tiles * T;
-        CUtensorMap mq, mk, mv;
-        int rc = tcore::maps(p, mq, mk, mv);
-        if (rc == FR_OK) rc = plan.tiles == 2 ? tcore::launch<2>(mq, mk, mv, p, plan.ctas, stream) : tcore::launch<1>(mq, mk, mv, p, plan.ctas, stream);
+        p.prefix_ctas = plan.whole ? 0 : plan.tiles * nkv * plan.prefix_splits;
+        p.covered = plan.own_tiles * (tcore::ROWS / (nq / nkv));
+        const int rc = tcore::launch(p, plan.ctas, stream);
         if (rc != FR_OK) return rc;
     } else {
         const int rc = dtype == FR_F32 ? launch_rows<float>(p, stream) : launch_rows<bf16>(p, stream);
@@ -869,9 +820,11 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     }
     *launches = 1;
     if (plan.parts > 1) {
-        const dim3 grid((unsigned)(((long long)rows * nq + 3) / 4));
-        if (dtype == FR_F32) FR_CUDA(fr_launch(merge_kernel<float>, grid, dim3(128), 0, stream, p));
-        else FR_CUDA(fr_launch(merge_kernel<bf16>, grid, dim3(128), 0, stream, p));
+        const dim3 grid((unsigned)((long long)rows * nq));
+        if (dtype == FR_F32 && hd % 4 == 0) FR_CUDA(fr_launch(merge_kernel<float, 4>, grid, dim3(128), 0, stream, p));
+        else if (dtype == FR_F32) FR_CUDA(fr_launch(merge_kernel<float, 1>, grid, dim3(256), 0, stream, p));
+        else if (hd % 4 == 0) FR_CUDA(fr_launch(merge_kernel<bf16, 4>, grid, dim3(128), 0, stream, p));
+        else FR_CUDA(fr_launch(merge_kernel<bf16, 1>, grid, dim3(256), 0, stream, p));
         FR_CHECK_LAUNCH("attention_shared (merge)");
         *launches = 2;
     }
