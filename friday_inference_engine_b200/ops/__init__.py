@@ -61,9 +61,9 @@ def _c_ints(values):
 
 
 def _sections(sections):
-    """(host array, number) of the sections' pairs"""
+    """(host array, number of sections, pairs in all)"""
     try:
-        s = tuple(int(n) for n in sections)
+        s = tuple(map(int, sections))
     except (TypeError, ValueError):
         raise native.KernelError("sections are numbers of pairs, one per axis, got %r" % (sections,)) from None
     if not 1 <= len(s) <= 4 or min(s) < 0 or sum(s) < 1:
@@ -117,6 +117,7 @@ class CudaOps:
 
     def __init__(self, device=0):
         self.device = int(device)
+        self._floats_of = {}                       # attention_shared: floats of scratch by a call's sizes
         self._h = c_void_p()
         native.call("friday_ops_new", int(device), None, byref(self._h))
 
@@ -267,49 +268,59 @@ class CudaOps:
         return s.value
 
     # -- a batch that shares a long prefix, positions with several axes ----
-    # These run on torch's current stream; what a call needs of scratch is torch's, so that a captured graph has its own.
+    # These run on torch's current stream; what a call needs of scratch is torch's, so that a captured graph has its own.  (Their
+    # checks are written to cost little: a step of a few rows is over in the time of some thirty Python calls.)
     def _stream(self):
         import torch
         return torch._C._cuda_getCurrentRawStream(self.device)
 
-    def _on_device(self, what, **tensors):
-        for name, t in tensors.items():
-            if t is not None and (not t.is_cuda or t.get_device() != self.device):
-                raise native.KernelError("%s: %s is on %s, these operations are cuda:%d's" % (what, name, t.device, self.device))
-
-    def _whole_numbers(self, what, at_least, **tensors):
-        """Tensors that kernels index as plain int32 arrays."""
+    def _row_tensor(self, what, name, t):
+        """FridayTensor of rows of float32 or bfloat16 on this device"""
         import torch
-        self._on_device(what, **tensors)
-        for name, t in tensors.items():
-            if t.dtype != torch.int32 or not t.is_contiguous():
-                raise native.KernelError("%s: %s must be contiguous int32, got %s with strides %s" % (what, name, t.dtype, t.stride()))
-            if t.numel() < at_least:
-                raise native.KernelError("%s: %s has %d numbers, %d are needed" % (what, name, t.numel(), at_least))
+        if t.get_device() != self.device:
+            raise native.KernelError("%s: %s is on %s, these operations are cuda:%d's" % (what, name, t.device, self.device))
+        code = _codes().get(t.dtype, 2)
+        if code > 1 or t.dim() != 2:
+            raise native.KernelError("%s: %s must be rows of float32 or bfloat16, got %s %s" % (what, name, t.dtype, tuple(t.shape)))
+        rows, columns = t.shape
+        ld, inner = t.stride()
+        if (inner != 1 and columns > 1) or (rows > 1 and ld < columns):
+            raise native.KernelError("%s: %s needs unit inner stride and rows apart, got strides %s" % (what, name, t.stride()))
+        return native.Tensor(t.data_ptr(), code, 2, (rows, columns), ld if rows > 1 else columns)
+
+    def _numbers(self, what, name, t, at_least):
+        """The address of what kernels index as a plain int32 array on this device"""
+        import torch
+        if t.dtype != torch.int32 or t.get_device() != self.device or not t.is_contiguous() or t.numel() < at_least:
+            raise native.KernelError("%s: %s must be at least %d contiguous int32 numbers on cuda:%d, got %s %s with strides %s on %s"
+                                     % (what, name, at_least, self.device, t.dtype, tuple(t.shape), t.stride(), t.device))
+        return t.data_ptr()
 
     def _axes(self, what, rows, positions, denom, sections):
         import torch
         array, axes, pairs = _sections(sections)
-        self._whole_numbers(what, rows * axes, positions=positions)
-        if positions.dim() != 2 or positions.shape[0] != rows or positions.shape[1] != axes:
+        if tuple(positions.shape) != (rows, axes):
             raise native.KernelError("%s: positions must be [%d rows, %d axes], got %s" % (what, rows, axes, tuple(positions.shape)))
-        self._on_device(what, denom=denom)
-        if denom.dtype != torch.float32 or not denom.is_contiguous() or denom.numel() != pairs:
-            raise native.KernelError("%s: denom must be %d contiguous float32 numbers, one per pair" % (what, pairs))
-        return array, axes
+        if denom.dtype != torch.float32 or denom.get_device() != self.device or not denom.is_contiguous() or denom.numel() != pairs:
+            raise native.KernelError("%s: denom must be %d contiguous float32 numbers on cuda:%d, one per pair" % (what, pairs, self.device))
+        return self._numbers(what, "positions", positions, 0), denom.data_ptr(), array, axes
 
-    def _pools(self, what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim):
-        self._on_device(what, k_pool=k_pool, v_pool=v_pool)
-        if k_pool.dtype not in _codes() or k_pool.dtype != v_pool.dtype:
-            raise native.KernelError("%s: pools of %s and %s" % (what, k_pool.dtype, v_pool.dtype))
-        for pool in (k_pool, v_pool):
-            if pool.dim() != 4 or not pool.is_contiguous() or tuple(pool.shape[1:]) != (page_size, n_kv_heads, head_dim) or pool.shape[0] < 1:
-                raise native.KernelError("%s: pools must be contiguous [pages, %d, %d, %d], got %s" % (what, page_size, n_kv_heads, head_dim, tuple(pool.shape)))
-        if k_pool.shape[0] != v_pool.shape[0] or k_pool.data_ptr() == v_pool.data_ptr():
-            raise native.KernelError("%s: keys and values need pools of their own with the same number of pages" % what)
-        self._whole_numbers(what, 0, block_table=block_table)
+    def _pools(self, what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim, write):
+        """FridayKV of pools [pages, page_size, n_kv_heads, head_dim] and a block table [sequences, pages]"""
+        code = _codes().get(k_pool.dtype, 2)
+        shape = k_pool.shape
+        if code > 1 or v_pool.dtype != k_pool.dtype or v_pool.shape != shape or tuple(shape) != (shape[0], page_size, n_kv_heads, head_dim) or shape[0] < 1:
+            raise native.KernelError("%s: pools must be [pages, %d, %d, %d] of float32 or bfloat16, got %s %s and %s %s"
+                                     % (what, page_size, n_kv_heads, head_dim, k_pool.dtype, tuple(shape), v_pool.dtype, tuple(v_pool.shape)))
+        if not (k_pool.is_contiguous() and v_pool.is_contiguous() and k_pool.get_device() == v_pool.get_device() == self.device):
+            raise native.KernelError("%s: pools must be contiguous and on cuda:%d" % (what, self.device))
+        k, v = k_pool.data_ptr(), v_pool.data_ptr()
+        if k == v:
+            raise native.KernelError("%s: keys and values need pools of their own" % what)
+        table = self._numbers(what, "block_table", block_table, 0)
         if block_table.dim() != 2:
             raise native.KernelError("%s: the block table is [sequences, pages], got %s" % (what, tuple(block_table.shape)))
+        return native.KV(k, v, shape[0], table, block_table.shape[1], page_size, 0, n_kv_heads, head_dim, code, write)
 
     def rotate_axes(self, x, positions, denom, sections, heads, head_dim, interleaved=False, neighbours=False, out=None):
         """The first `heads` heads of every row of x [rows, >= heads * head_dim], turned: pair i of a head by
@@ -317,47 +328,43 @@ class CudaOps:
         with `interleaved` in turn: pair i belongs to axis i mod n if i < n * sections[i mod n], else to axis 0.  A pair is
         (i, i + pairs), with `neighbours` (2i, 2i + 1); dimensions behind the pairs stay.  out [rows, heads * head_dim] may be x's own
         columns (None: a new tensor).  positions int32 [rows, axes], denom float32 [pairs], not zero.  -> out"""
-        import torch
+        what = "rotate_axes"
         heads, head_dim = int(heads), int(head_dim)
-        self._on_device("rotate_axes", x=x, out=out)
-        if x.dim() != 2:
-            raise native.KernelError("rotate_axes: rows [rows, columns] are wanted, got %s" % (tuple(x.shape),))
-        array, axes = self._axes("rotate_axes", x.shape[0], positions, denom, sections)
+        xt = self._row_tensor(what, "x", x)
+        rows = xt.shape[0]
+        pos, den, array, axes = self._axes(what, rows, positions, denom, sections)
         if out is None:
-            out = torch.empty((x.shape[0], max(heads, 0) * max(head_dim, 0)), dtype=x.dtype, device=x.device)
-        if x.shape[0] == 0:
+            out = x.new_empty((rows, max(heads, 0) * max(head_dim, 0)))
+        ot = self._row_tensor(what, "out", out)
+        if rows == 0:
             return out
-        native.call("friday_ops_rotate_axes", self._h, _t(x), _t(out), positions.data_ptr(), denom.data_ptr(), array, axes,
-                    1 if interleaved else 0, 1 if neighbours else 0, heads, head_dim, self._stream())
+        native.call("friday_ops_rotate_axes", self._h, xt, ot, pos, den, array, axes, 1 if interleaved else 0, 1 if neighbours else 0,
+                    heads, head_dim, self._stream())
         return out
 
     def rope_axes_kv_write(self, qkv, row_seq, row_pos, positions, denom, sections, n_heads, n_kv_heads, head_dim, k_pool, v_pool,
                            block_table, page_size, interleaved=False, neighbours=False, q_out=None):
         """Rows [queries | keys | values] of qkv: the queries turned (see rotate_axes) into q_out [rows, n_heads * head_dim] (may be
         qkv's own query columns; None: a new tensor), keys turned and values as they are to the cache's row of (row_seq, row_pos):
-        page block_table[row_seq][row_pos / page_size], row row_pos mod page_size.  qkv itself is left as it was.  Rows whose row_seq
+        page block_table[row_seq][row_pos / page_size], row row_pos mod page_size.  Nothing else of qkv changes.  Rows whose row_seq
         is negative are left alone; a row whose place the table does not name only gets its queries.  No two rows of a call may name
         the same place.  -> q_out"""
-        import torch
         what = "rope_axes_kv_write"
         n_heads, n_kv_heads, head_dim, page_size = int(n_heads), int(n_kv_heads), int(head_dim), int(page_size)
-        self._on_device(what, qkv=qkv, q_out=q_out)
-        if qkv.dim() != 2:
-            raise native.KernelError("%s: rows [rows, columns] are wanted, got %s" % (what, tuple(qkv.shape)))
-        rows = qkv.shape[0]
-        array, axes = self._axes(what, rows, positions, denom, sections)
-        self._whole_numbers(what, rows, row_seq=row_seq, row_pos=row_pos)
-        self._pools(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim)
+        xt = self._row_tensor(what, "qkv", qkv)
+        rows = xt.shape[0]
+        pos, den, array, axes = self._axes(what, rows, positions, denom, sections)
+        kv = self._pools(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim, 1)
+        seq, place = self._numbers(what, "row_seq", row_seq, rows), self._numbers(what, "row_pos", row_pos, rows)
         if q_out is None:
-            q_out = torch.empty((rows, max(n_heads, 0) * head_dim), dtype=qkv.dtype, device=qkv.device)
+            q_out = qkv.new_empty((rows, max(n_heads, 0) * head_dim))
+        qt = self._row_tensor(what, "q_out", q_out) if n_heads > 0 else None
         if rows == 0 or block_table.shape[0] == 0:
             return q_out
-        if block_table.shape[1] == 0:
+        if kv.table_width == 0:
             raise native.KernelError("%s: the block table is empty" % what)
-        kv = _kv(k_pool, v_pool, block_table, page_size)
-        native.call("friday_ops_rope_axes_kv_write", self._h, _t(qkv), _t(q_out) if n_heads > 0 else None, row_seq.data_ptr(),
-                    row_pos.data_ptr(), positions.data_ptr(), denom.data_ptr(), array, axes, 1 if interleaved else 0,
-                    1 if neighbours else 0, n_heads, n_kv_heads, head_dim, byref(kv), block_table.shape[0], self._stream())
+        native.call("friday_ops_rope_axes_kv_write", self._h, xt, qt, seq, place, pos, den, array, axes, 1 if interleaved else 0,
+                    1 if neighbours else 0, n_heads, n_kv_heads, head_dim, kv, block_table.shape[0], self._stream())
         return q_out
 
     def attention_shared(self, q, q_stride, out, k_pool, v_pool, prefix_table, prefix_len, block_table, page_size, row_seq, row_pos,
@@ -372,39 +379,44 @@ class CudaOps:
         device): the rows of sequence s are seq_start[s] and the seq_qlen[s] - 1 after it, row_seq says so too.  max_q_len bounds
         seq_qlen; max_kv_len is a bound on the positions that only shares the work out.  prefix_len is a number of the host's: a
         captured graph keeps it."""
-        import torch
         what = "attention_shared"
         n_heads, n_kv_heads, head_dim, page_size = int(n_heads), int(n_kv_heads), int(head_dim), int(page_size)
-        prefix_len, window, rows = int(prefix_len), int(window or 0), out.shape[0]
-        self._on_device(what, q=q, out=out)
-        self._pools(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim)
-        if q.dim() != 2 or out.dim() != 2 or (rows > 1 and q.stride(0) != q_stride):
-            raise native.KernelError("%s: rows of queries whose stride is q_stride and rows of results are wanted, got strides %s and %s, q_stride %d"
-                                     % (what, q.stride(), out.stride(), q_stride))
-        self._whole_numbers(what, rows, row_seq=row_seq, row_pos=row_pos)
+        prefix_len, window, q_stride = int(prefix_len), int(window or 0), int(q_stride)
+        qt, ot = self._row_tensor(what, "q", q), self._row_tensor(what, "out", out)
+        rows = ot.shape[0]
+        kv = self._pools(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim, 0)
+        if rows > 1 and qt.ld != q_stride:
+            raise native.KernelError("%s: rows of queries %d apart, q_stride %d" % (what, qt.ld, q_stride))
         n_seqs, max_q_len, max_kv_len = int(geometry.n_seqs), int(geometry.max_q_len), int(geometry.max_kv_len)
         if block_table.shape[0] < n_seqs:
             raise native.KernelError("%s: %d sequences, a block table of %d" % (what, n_seqs, block_table.shape[0]))
+        g = native.Geometry(rows, n_seqs, max_q_len, max_kv_len, 0, self._numbers(what, "row_seq", row_seq, rows),
+                            self._numbers(what, "row_pos", row_pos, rows), self._numbers(what, "seq_start", geometry.seq_start, n_seqs),
+                            self._numbers(what, "seq_qlen", geometry.seq_qlen, n_seqs), None)
+        prefix = None
         if prefix_len > 0:
             if prefix_table is None:
                 raise native.KernelError("%s: a prefix of %d needs its pages" % (what, prefix_len))
-            self._whole_numbers(what, -(-prefix_len // page_size), prefix_table=prefix_table)
-        self._whole_numbers(what, n_seqs, seq_start=geometry.seq_start, seq_qlen=geometry.seq_qlen)
+            prefix = self._numbers(what, "prefix_table", prefix_table, -(-prefix_len // page_size))
         if rows == 0 or n_seqs <= 0:
             return
-        floats = c_int64()
-        code = _codes()[k_pool.dtype]
-        native.call("friday_ops_attention_shared_floats", self._h, rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads,
-                    head_dim, page_size, window, code, byref(floats))
-        scratch = torch.empty((floats.value,), dtype=torch.float32, device=out.device) if floats.value else None
-        g = native.Geometry()
-        g.rows, g.n_seqs, g.max_q_len, g.max_kv_len = rows, n_seqs, max_q_len, max_kv_len
-        g.row_seq, g.row_pos = row_seq.data_ptr(), row_pos.data_ptr()
-        g.seq_start, g.seq_qlen = geometry.seq_start.data_ptr(), geometry.seq_qlen.data_ptr()
-        kv = _kv(k_pool, v_pool, block_table, page_size, write=False)
-        native.call("friday_ops_attention_shared", self._h, _t(q), int(q_stride), _t(out), byref(kv),
-                    prefix_table.data_ptr() if prefix_len > 0 else None, prefix_len, byref(g), n_heads, n_kv_heads, head_dim, window,
-                    float(scale), scratch.data_ptr() if scratch is not None else None, floats.value, self._stream())
+        floats = self._shared_floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, page_size, window, kv.dtype)
+        scratch = None
+        if floats:
+            import torch
+            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        native.call("friday_ops_attention_shared", self._h, qt, q_stride, ot, kv, prefix, prefix_len, g, n_heads, n_kv_heads, head_dim,
+                    window, float(scale), scratch.data_ptr() if floats else None, floats, self._stream())
+
+    def _shared_floats(self, *sizes):
+        got = self._floats_of.get(sizes)
+        if got is None:
+            n = c_int64()
+            native.call("friday_ops_attention_shared_floats", self._h, *sizes, byref(n))
+            if len(self._floats_of) >= 4096:                  # (sizes of a step: a few of them come again and again)
+                self._floats_of.clear()
+            got = self._floats_of[sizes] = n.value
+        return got
 
     # -- one attention kernel's launcher, called directly with chosen arguments (tests of that kernel alone) -----
     def _test_buffers(self, device):

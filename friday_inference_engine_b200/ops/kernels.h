@@ -227,9 +227,9 @@ struct AttentionTc {
 };
 struct RopeAxes {
     last_error_fn last_error;
-    int (*rotate)(const void*, long long, void*, long long, int, int, int, const int*, int, const float*, const int*, int, int, int, cudaStream_t);
+    int (*rotate)(const void*, long long, void*, long long, int, int, int, const int*, int, const float*, const int*, int, int, int*, int, cudaStream_t);
     int (*append)(const void*, long long, void*, long long, int, int, int, int, const int*, const int*, const int*, int, const float*, const int*, int, int,
-                  void*, void*, int, int, const int*, int, int, int, cudaStream_t);
+                  void*, void*, int, int, const int*, int, int, int*, int, cudaStream_t);
 };
 struct AttentionShared {
     last_error_fn last_error;

@@ -1718,18 +1718,18 @@ void Ops::attention(const Tensor& q, int64_t q_stride, Tensor& out, const CacheV
 
 // ------------------------------------------------------------------ a shared prefix, positions with several axes
 namespace {
-// Two sets of rows of `n` columns each: true if a number could belong to both.  The same first column and row length (in place), or
-// columns beside one another of rows of one length, are apart.
-bool rows_collide(const Tensor& a, const Tensor& b, int64_t n, bool same_is_fine) {
+// Rows of `na` and of `nb` columns: true if a number could belong to both.  The same first column and row length (in place), or columns
+// beside one another of rows of one length, are apart.
+bool rows_collide(const Tensor& a, int64_t na, const Tensor& b, int64_t nb, bool same_is_fine) {
     if (a.rows() <= 0 || b.rows() <= 0) return false;
     const int64_t es = (int64_t)dtype_size(a.dtype);
     const char *pa = (const char*)a.data, *pb = (const char*)b.data;
-    const int64_t la = ((a.rows() - 1) * a.ld + n) * es, lb = ((b.rows() - 1) * b.ld + n) * es;
+    const int64_t la = ((a.rows() - 1) * a.ld + na) * es, lb = ((b.rows() - 1) * b.ld + nb) * es;
     if (pa + la <= pb || pb + lb <= pa) return false;
     if (pa == pb && same_is_fine && (a.ld == b.ld || a.rows() == 1)) return false;
     if (a.ld != b.ld || (pb - pa) % es) return true;
     const int64_t step = (((pb - pa) / es) % a.ld + a.ld) % a.ld;
-    return step < n || step > a.ld - n;
+    return step < na || step > a.ld - nb;
 }
 
 void check_rows(const char* what, const Tensor& t, int64_t columns) {
@@ -1751,11 +1751,11 @@ void Ops::rotate_axes(const Tensor& x, Tensor& out, const int* positions, const 
     check_axes("rotate_axes", spec, positions);
     if (out.rows() != x.rows() || out.dtype != x.dtype) throw KernelError("rotate_axes: the result needs the rows and the dtype of what is turned");
     if (x.rows() > 0x7fffffff) throw KernelError("rotate_axes: too many rows");
-    if (rows_collide(x, out, n, true)) throw KernelError("rotate_axes: the result overlaps what is turned and is not the same columns");
+    if (rows_collide(x, n, out, n, true)) throw KernelError("rotate_axes: the result overlaps what is turned and is not the same columns");
     const auto& k = kernels::rope_axes();
     std::unique_ptr<Timed> t(place ? nullptr : new Timed(*this, Other));
     const int rc = k.rotate(x.data, x.ld, out.data, out.ld, (int)x.rows(), heads, head_dim, positions, (int)spec.sections.size(), spec.denominators,
-                            spec.sections.data(), spec.interleaved, spec.neighbours, code(x.dtype), place ? place->stream : stream_);
+                            spec.sections.data(), spec.interleaved, spec.neighbours, (int*)status_.get(), code(x.dtype), place ? place->stream : stream_);
     if (rc != 0) throw KernelError(std::string("rotate_axes: ") + k.last_error());
     __atomic_add_fetch(&launches_, x.rows() > 0 ? 1 : 0, __ATOMIC_RELAXED);
 }
@@ -1776,8 +1776,8 @@ void Ops::rope_axes_kv_write(const Tensor& qkv, Tensor* q_out, const int* row_se
         if (!q_out) throw KernelError("rope_axes_kv_write: a place for the turned queries is needed");
         check_rows("rope_axes_kv_write", *q_out, (int64_t)n_heads * head_dim);
         if (q_out->rows() != qkv.rows() || q_out->dtype != qkv.dtype) throw KernelError("rope_axes_kv_write: the queries need the rows and the dtype of qkv");
-        Tensor q = qkv;                                                    // the keys and values are read too: only the query columns may be the same
-        if (rows_collide(q, *q_out, (int64_t)(n_heads + 2 * n_kv_heads) * head_dim, false) &&
+        // (the keys and values are read too: only the query columns may be the same)
+        if (rows_collide(qkv, (int64_t)(n_heads + 2 * n_kv_heads) * head_dim, *q_out, (int64_t)n_heads * head_dim, false) &&
             !(q_out->data == qkv.data && (q_out->ld == qkv.ld || qkv.rows() == 1)))
             throw KernelError("rope_axes_kv_write: the turned queries overlap qkv and are not its query columns");
     }
@@ -1787,7 +1787,7 @@ void Ops::rope_axes_kv_write(const Tensor& qkv, Tensor* q_out, const int* row_se
     const int rc = k.append(qkv.data, qkv.ld, n_heads > 0 ? q_out->data : nullptr, n_heads > 0 ? q_out->ld : 0, (int)qkv.rows(), n_heads, n_kv_heads,
                             head_dim, row_seq, row_pos, positions, (int)spec.sections.size(), spec.denominators, spec.sections.data(),
                             spec.interleaved, spec.neighbours, view.k_pool, view.v_pool, view.pool_pages, view.page_size, view.block_table,
-                            n_seqs, view.table_width, code(qkv.dtype), place ? place->stream : stream_);
+                            n_seqs, view.table_width, (int*)status_.get(), code(qkv.dtype), place ? place->stream : stream_);
     if (rc != 0) throw KernelError(std::string("rope_axes_kv_write: ") + k.last_error());
     __atomic_add_fetch(&launches_, qkv.rows() > 0 ? 1 : 0, __ATOMIC_RELAXED);
 }
@@ -1818,7 +1818,7 @@ void Ops::attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const
         throw KernelError("attention_shared: the step's geometry (rows' sequences and positions, the sequences' rows) is needed");
     Tensor q_rows = q;
     q_rows.shape[0] = rows;
-    if (rows_collide(q_rows, out, n, false)) throw KernelError("attention_shared: the result overlaps the queries");
+    if (rows_collide(q_rows, n, out, n, false)) throw KernelError("attention_shared: the result overlaps the queries");
     const auto& k = kernels::attention_shared();
     const int64_t floats = attention_shared_floats(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, view.page_size, window, out.dtype);
     if (place && place->scratch_floats < floats) throw KernelError(format("attention_shared: %lld floats of scratch are needed", (long long)floats));

@@ -90,7 +90,65 @@ def test_rotation_of_many_rows():
     assert ops.rotate_axes(x[:0], pos[:0], ladder(40), sections, heads, hd).shape == (0, heads * hd)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,heads,hd,sections,interleaved,neighbours,beside", [
+    (3001, 24, 72, [18, 18], False, False, 0), (2500, 24, 72, [16, 12, 8], True, True, 8), (9000, 8, 36, [9, 9], False, False, 0), (9000, 8, 36, [9, 9], False, True, 16),
+    (4099, 12, 64, [8, 4, 4], False, False, 0), (1500, 6, 256, [48, 40, 40], True, False, 0), (70000, 1, 32, [16], False, False, 0), (60000, 1, 40, [6, 7], False, True, 0),
+    (700, 40, 128, [24, 20, 20], False, False, 24)])
+def test_rotation_of_rows_by_the_megabyte(dtype, rows, heads, hd, sections, interleaved, neighbours, beside):
+    x = rnd((rows, (heads * hd + beside)), dtype, 45)
+    keep = x.clone()
+    pos = torch.randint(0, 9000, (rows, len(sections)), generator=torch.Generator().manual_seed(46), dtype=torch.int32).to(DEV)
+    denom = ladder(sum(sections))
+    out = ops.rotate_axes(x, pos, denom, sections, heads, hd, interleaved=interleaved, neighbours=neighbours)
+    ref, err = sp.turned(x[:, :heads * hd].double().reshape(rows, heads, hd), pos, denom, sections, interleaved, neighbours)
+    within(out, ref.flatten(1), err.flatten(1), dtype, "many rows")
+    half = sum(sections)
+    assert torch.equal(out.view(rows, heads, hd)[..., 2 * half:], keep[:, :heads * hd].reshape(rows, heads, hd)[..., 2 * half:])
+    ops.rotate_axes(x[:, :heads * hd], pos, denom, sections, heads, hd, interleaved=interleaved, neighbours=neighbours, out=x[:, :heads * hd])
+    assert torch.equal(x[:, :heads * hd], out) and torch.equal(x[:, heads * hd:], keep[:, heads * hd:])
+
+
 # ------------------------------------------------------------------ append
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("nq,nkv,hd,sections,neighbours,beside", [(28, 4, 128, [16, 24, 24], False, 0), (3, 1, 32, [4, 4], True, 8), (8, 8, 72, [12, 12, 12], False, 0), (0, 2, 64, [16], False, 0)])
+def test_append_of_rows_by_the_megabyte(dtype, nq, nkv, hd, sections, neighbours, beside):
+    """Rows without a sequence, places that no page has, and pages in any order among many rows."""
+    width = (nq + 2 * nkv) * hd
+    rows = (3 << 20) // (width * 2) + 37
+    pages = rows // PAGE + 9
+    wide = rnd((rows, width + beside), dtype, 47)
+    qkv = wide[:, :width]
+    g = torch.Generator().manual_seed(48)
+    table = torch.randperm(pages, generator=g)[:pages // 2 * 2].to(torch.int32).view(2, -1).contiguous()
+    order = torch.randperm(2 * table.shape[1] * PAGE, generator=g)[:rows]
+    seq, place = (order % 2).to(torch.int32), (order // 2).to(torch.int32)
+    seq[5::97] = -1
+    place[7::101] = table.shape[1] * PAGE + 3
+    table[1, 1] = -1
+    seq, place, table = seq.to(DEV), place.to(DEV), table.to(DEV)
+    pos = torch.randint(0, 9000, (rows, len(sections)), generator=g, dtype=torch.int32).to(DEV)
+    denom = ladder(sum(sections))
+    kp = torch.full((pages, PAGE, nkv, hd), 3.0, dtype=dtype, device=DEV)
+    vp = kp.clone()
+    q = torch.full((rows, nq * hd), 9.0, dtype=dtype, device=DEV)
+    ops.rope_axes_kv_write(qkv, seq, place, pos, denom, sections, nq, nkv, hd, kp, vp, table, PAGE, neighbours=neighbours, q_out=q)
+    heads = qkv.double().reshape(rows, nq + 2 * nkv, hd)
+    ref, err = sp.turned(heads[:, :nq + nkv], pos, denom, sections, False, neighbours)
+    live = seq >= 0
+    if nq:
+        within(q[live], ref[live][:, :nq].flatten(1), err[live][:, :nq].flatten(1), dtype, "queries")
+        assert bool((q[~live] == 9.0).all())
+    page = torch.where(live & (place < table.shape[1] * PAGE), table[seq.clamp(min=0).long(), (place // PAGE).clamp(max=table.shape[1] - 1).long()], -1)
+    kept = page >= 0
+    flat = (page.long() * PAGE + place.long() % PAGE)[kept]
+    within(kp.flatten(0, 1)[flat].flatten(1), ref[kept][:, nq:].flatten(1), err[kept][:, nq:].flatten(1), dtype, "keys")
+    assert torch.equal(vp.flatten(0, 1)[flat], qkv.reshape(rows, -1, hd)[kept][:, nq + nkv:])
+    others = torch.ones(pages * PAGE, dtype=torch.bool, device=DEV)
+    others[flat] = False
+    assert bool((kp.flatten(0, 1)[others] == 3.0).all()) and bool((vp.flatten(0, 1)[others] == 3.0).all())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("nq,nkv,hd,sections,interleaved,neighbours", [
     (5, 2, 48, [8, 8, 8], False, False), (28, 4, 128, [16, 24, 24], False, False), (40, 8, 128, [24, 20, 20], True, False),
@@ -150,6 +208,23 @@ def test_append_with_equal_positions_agrees_with_the_one_axis_rotation(dtype):
     for a, b in ((q, qkv[:, :nq * hd]), (kp, kp2)):
         assert bool(((a.double() - b.double()).abs() <= step * b.double().abs() + 70 * 2.0 ** -22).all())
     assert torch.equal(vp, vp2)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5])
+def test_append_between_tensors_side_by_side_in_memory(rows):
+    """Rows and turned queries that touch, and turned queries in columns behind the rows' own, are not on one another."""
+    nq, nkv, hd = 6, 2, 32
+    width = (nq + 2 * nkv) * hd
+    buf = rnd((rows * (width + nq * hd),), BF, 44)
+    seq, place = torch.zeros(rows, dtype=torch.int32, device=DEV), torch.arange(rows, dtype=torch.int32, device=DEV)
+    pos = torch.stack((place + 3, place), 1).contiguous()
+    kp, vp = (torch.zeros((2, PAGE, nkv, hd), dtype=BF, device=DEV) for _ in range(2))
+    args = (seq, place, pos, ladder(16), [8, 8], nq, nkv, hd, kp, vp, torch.tensor([[1]], dtype=torch.int32, device=DEV), PAGE)
+    apart, touching = buf[:rows * width].view(rows, width), buf[rows * width:].view(rows, nq * hd)
+    want = ops.rope_axes_kv_write(apart.clone(), *args)
+    assert torch.equal(ops.rope_axes_kv_write(apart, *args, q_out=touching), want)
+    wide = torch.cat((apart, torch.zeros((rows, nq * hd), dtype=BF, device=DEV)), 1)
+    assert torch.equal(ops.rope_axes_kv_write(wide[:, :width], *args, q_out=wide[:, width:]), want)
 
 
 def test_append_of_many_rows_far_into_a_large_pool():
