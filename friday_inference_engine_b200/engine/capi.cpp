@@ -182,21 +182,6 @@ CacheView view_of(const FridayKV* kv) {
     return v;
 }
 
-StepContext context_of(const FridayGeometry* g) {
-    StepContext ctx;
-    ctx.rows = g->rows;
-    ctx.n_seqs = g->n_seqs;
-    ctx.max_q_len = g->max_q_len;
-    ctx.max_kv_len = g->max_kv_len;
-    ctx.decode = g->decode != 0;
-    ctx.row_seq = g->row_seq;
-    ctx.row_pos = g->row_pos;
-    ctx.seq_start = g->seq_start;
-    ctx.seq_qlen = g->seq_qlen;
-    ctx.seq_pos0 = g->seq_pos0;
-    return ctx;
-}
-
 // The handle's device for the length of a call; the thread's own afterwards.
 struct OnDevice {
     int before = -1;
@@ -209,6 +194,32 @@ struct OnDevice {
         if (before >= 0) cudaSetDevice(before);
     }
 };
+
+Tensor rows_at(const void* data, int dtype, int64_t rows, int64_t cols, int64_t ld) {
+    Tensor t;
+    t.data = (void*)data;
+    t.dtype = (DType)dtype;
+    t.ndim = 2;
+    t.shape[0] = rows;
+    t.shape[1] = cols;
+    t.ld = rows > 1 ? ld : cols;
+    return t;
+}
+
+CacheView cache_at(void* k_pool, void* v_pool, int pool_pages, int page, int nkv, int hd, int dtype, const int* block_table, int table_width) {
+    CacheView v;
+    v.kind = CacheRequest::KV;
+    v.k_pool = k_pool;
+    v.v_pool = v_pool;
+    v.pool_pages = pool_pages;
+    v.block_table = block_table;
+    v.table_width = table_width;
+    v.page_size = page;
+    v.n_kv_heads = nkv;
+    v.head_dim = hd;
+    v.dtype = (DType)dtype;
+    return v;
+}
 
 Ops::AxesSpec axes_of(const int* sections, int axes, int interleaved, int neighbours, const float* denominators) {
     if (!sections || axes < 1 || axes > 4) throw KernelError(format("1 to 4 sections are wanted, got %d", axes));
@@ -789,28 +800,45 @@ FR_API int friday_ops_linear_swiglu(void* h, const FridayTensor* x, const Friday
 FR_API int friday_ops_attention(void* h, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
                                 const FridayGeometry* g, int nq, int nkv, int hd, int window, float scale) {
     GUARD({
-        const StepContext ctx = context_of(g);
+        StepContext ctx;
+        ctx.rows = g->rows;
+        ctx.n_seqs = g->n_seqs;
+        ctx.max_q_len = g->max_q_len;
+        ctx.max_kv_len = g->max_kv_len;
+        ctx.decode = g->decode != 0;
+        ctx.row_seq = g->row_seq;
+        ctx.row_pos = g->row_pos;
+        ctx.seq_start = g->seq_start;
+        ctx.seq_qlen = g->seq_qlen;
+        ctx.seq_pos0 = g->seq_pos0;
         ((OpsHandle*)h)->begin().attention(*T(q), q_stride, *T(out), view_of(kv), ctx, nq, nkv, hd, window, scale);
     })
 }
-FR_API int friday_ops_rotate_axes(void* h, const FridayTensor* x, FridayTensor* out, const int* positions, const float* denominators,
+FR_API int friday_ops_rotate_axes(void* h, const void* x, int64_t x_rows, int64_t x_cols, int64_t x_ld, void* out, int64_t out_rows,
+                                  int64_t out_cols, int64_t out_ld, int dtype, const int* positions, const float* denominators,
                                   const int* sections, int axes, int interleaved, int neighbours, int heads, int head_dim, void* stream) {
     GUARD({
         Ops& ops = *((OpsHandle*)h)->ops;
         OnDevice on(ops.device());
         const Ops::Place place{(cudaStream_t)stream, nullptr, 0};
-        ops.rotate_axes(*T(x), *T(out), positions, axes_of(sections, axes, interleaved, neighbours, denominators), heads, head_dim, &place);
+        Tensor o = rows_at(out, dtype, out_rows, out_cols, out_ld);
+        ops.rotate_axes(rows_at(x, dtype, x_rows, x_cols, x_ld), o, positions, axes_of(sections, axes, interleaved, neighbours, denominators),
+                        heads, head_dim, &place);
     })
 }
-FR_API int friday_ops_rope_axes_kv_write(void* h, const FridayTensor* qkv, FridayTensor* q_out, const int* row_seq, const int* row_pos,
+FR_API int friday_ops_rope_axes_kv_write(void* h, const void* qkv, int64_t rows, int64_t cols, int64_t ld, void* q_out, int64_t q_rows,
+                                         int64_t q_cols, int64_t q_ld, int dtype, const int* row_seq, const int* row_pos,
                                          const int* positions, const float* denominators, const int* sections, int axes, int interleaved,
-                                         int neighbours, int nq, int nkv, int hd, const FridayKV* kv, int n_seqs, void* stream) {
+                                         int neighbours, int nq, int nkv, int hd, void* k_pool, void* v_pool, int pool_pages, int page,
+                                         const int* block_table, int n_seqs, int table_width, void* stream) {
     GUARD({
         Ops& ops = *((OpsHandle*)h)->ops;
         OnDevice on(ops.device());
         const Ops::Place place{(cudaStream_t)stream, nullptr, 0};
-        ops.rope_axes_kv_write(*T(qkv), q_out ? T(q_out) : nullptr, row_seq, row_pos, positions,
-                               axes_of(sections, axes, interleaved, neighbours, denominators), nq, nkv, hd, view_of(kv), n_seqs, &place);
+        Tensor q = rows_at(q_out, dtype, q_rows, q_cols, q_ld);
+        ops.rope_axes_kv_write(rows_at(qkv, dtype, rows, cols, ld), q_out ? &q : nullptr, row_seq, row_pos, positions,
+                               axes_of(sections, axes, interleaved, neighbours, denominators), nq, nkv, hd,
+                               cache_at(k_pool, v_pool, pool_pages, page, nkv, hd, dtype, block_table, table_width), n_seqs, &place);
     })
 }
 FR_API int friday_ops_attention_shared_floats(void* h, int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int nq, int nkv,
@@ -821,14 +849,29 @@ FR_API int friday_ops_attention_shared_floats(void* h, int rows, int n_seqs, int
         *floats = ops.attention_shared_floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, nq, nkv, hd, page, window, (DType)dtype);
     })
 }
-FR_API int friday_ops_attention_shared(void* h, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
-                                       const int* prefix_table, int prefix_len, const FridayGeometry* g, int nq, int nkv, int hd, int window,
-                                       float scale, float* scratch, int64_t scratch_floats, void* stream) {
+FR_API int friday_ops_attention_shared(void* h, const void* q, int64_t q_rows, int64_t q_cols, int64_t q_stride, void* out, int64_t rows,
+                                       int64_t out_cols, int dtype, const void* k_pool, const void* v_pool, int pool_pages, int page,
+                                       const int* prefix_table, int prefix_len, const int* block_table, int n_seqs, int table_width,
+                                       const int* row_seq, const int* row_pos, const int* seq_start, const int* seq_qlen, int max_q_len,
+                                       int max_kv_len, int nq, int nkv, int hd, int window, float scale, float* scratch,
+                                       int64_t scratch_floats, void* stream) {
     GUARD({
         Ops& ops = *((OpsHandle*)h)->ops;
         OnDevice on(ops.device());
         const Ops::Place place{(cudaStream_t)stream, scratch, scratch_floats};
-        ops.attention_shared(*T(q), q_stride, *T(out), view_of(kv), prefix_table, prefix_len, context_of(g), nq, nkv, hd, window, scale, &place);
+        StepContext ctx;
+        ctx.rows = (int)rows;
+        ctx.n_seqs = n_seqs;
+        ctx.max_q_len = max_q_len;
+        ctx.max_kv_len = max_kv_len;
+        ctx.row_seq = row_seq;
+        ctx.row_pos = row_pos;
+        ctx.seq_start = seq_start;
+        ctx.seq_qlen = seq_qlen;
+        Tensor o = rows_at(out, dtype, rows, out_cols, out_cols);
+        ops.attention_shared(rows_at(q, dtype, q_rows, q_cols, q_rows > 1 ? q_stride : q_cols), q_stride, o,
+                             cache_at((void*)k_pool, (void*)v_pool, pool_pages, page, nkv, hd, dtype, block_table, table_width), prefix_table,
+                             prefix_len, ctx, nq, nkv, hd, window, scale, &place);
     })
 }
 FR_API int friday_ops_sample(void* h, const FridayTensor* logits, const float* temperature, const int* streams,

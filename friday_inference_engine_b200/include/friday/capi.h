@@ -149,18 +149,26 @@ int friday_ops_attention(void* ops, const FridayTensor* q, int64_t q_stride, Fri
                          const FridayGeometry* geometry, int n_heads, int n_kv_heads, int head_dim, int window, float scale);
 /* Rotary positions with several axes, their append to the cache, attention of a batch with a shared prefix (friday::Ops::rotate_axes,
  * rope_axes_kv_write, attention_shared).  They run on the stream that is given, use nothing of the handle that another call could be
- * using, and leave the calling thread's current device as it was.  sections: host, [axes]; out, q_out and scratch are the caller's. */
-int friday_ops_rotate_axes(void* ops, const FridayTensor* x, FridayTensor* out, const int* positions, const float* denominators,
+ * using, and leave the calling thread's current device as it was.  Rows are given by address, rows, columns and row length (ld);
+ * dtype 0 float32, 1 bfloat16; sections: host, [axes]; pools [pages][page_size][n_kv_heads][head_dim]; block_table [n_seqs][table_width];
+ * results and scratch are the caller's. */
+int friday_ops_rotate_axes(void* ops, const void* x, int64_t x_rows, int64_t x_cols, int64_t x_ld, void* out, int64_t out_rows,
+                           int64_t out_cols, int64_t out_ld, int dtype, const int* positions, const float* denominators,
                            const int* sections, int axes, int interleaved, int neighbours, int heads, int head_dim, void* stream);
-int friday_ops_rope_axes_kv_write(void* ops, const FridayTensor* qkv, FridayTensor* q_out, const int* row_seq, const int* row_pos,
-                                  const int* positions, const float* denominators, const int* sections, int axes, int interleaved,
-                                  int neighbours, int n_heads, int n_kv_heads, int head_dim, const FridayKV* kv, int n_seqs, void* stream);
-/* floats of scratch that an attention_shared of these sizes needs (dtype: 0 float32, 1 bfloat16) */
+int friday_ops_rope_axes_kv_write(void* ops, const void* qkv, int64_t rows, int64_t cols, int64_t ld, void* q_out, int64_t q_rows,
+                                  int64_t q_cols, int64_t q_ld, int dtype, const int* row_seq, const int* row_pos, const int* positions,
+                                  const float* denominators, const int* sections, int axes, int interleaved, int neighbours, int n_heads,
+                                  int n_kv_heads, int head_dim, void* k_pool, void* v_pool, int pool_pages, int page_size,
+                                  const int* block_table, int n_seqs, int table_width, void* stream);
+/* floats of scratch that an attention_shared of these sizes needs */
 int friday_ops_attention_shared_floats(void* ops, int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix_len, int n_heads,
                                        int n_kv_heads, int head_dim, int page_size, int window, int dtype, int64_t* floats);
-int friday_ops_attention_shared(void* ops, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
-                                const int* prefix_table, int prefix_len, const FridayGeometry* geometry, int n_heads, int n_kv_heads,
-                                int head_dim, int window, float scale, float* scratch, int64_t scratch_floats, void* stream);
+int friday_ops_attention_shared(void* ops, const void* q, int64_t q_rows, int64_t q_cols, int64_t q_stride, void* out, int64_t rows,
+                                int64_t out_cols, int dtype, const void* k_pool, const void* v_pool, int pool_pages, int page_size,
+                                const int* prefix_table, int prefix_len, const int* block_table, int n_seqs, int table_width,
+                                const int* row_seq, const int* row_pos, const int* seq_start, const int* seq_qlen, int max_q_len,
+                                int max_kv_len, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float* scratch,
+                                int64_t scratch_floats, void* stream);
 int friday_ops_sample(void* ops, const FridayTensor* logits, const float* temperature, const int* streams, const int* steps,
                       uint64_t seed, const int* row_live, int* out);
 int friday_ops_plan(void* ops, int64_t rows, int64_t n, int64_t k, int* swapped, int* bn, int* splits);

@@ -91,7 +91,7 @@ class LoopHooks(Structure):
                 ("free_slot", FREE_HOOK)]
 
 
-P, I, F, S = c_void_p, c_int, c_float, c_char_p
+P, I, F, S, L = c_void_p, c_int, c_float, c_char_p, c_int64
 PP, PS, PI = POINTER(c_void_p), POINTER(c_char_p), POINTER(c_int)
 T = POINTER(Tensor)
 
@@ -152,10 +152,10 @@ _SIGNATURES = {
     "friday_ops_qkv_rope_write": [P, T, T, F, T, T, P, P, P, I, I, I, I, POINTER(KV), T],
     "friday_ops_linear_swiglu": [P, T, T, F, T, T],
     "friday_ops_attention": [P, T, c_int64, T, POINTER(KV), POINTER(Geometry), I, I, I, I, F],
-    "friday_ops_rotate_axes": [P, T, T, P, P, PI, I, I, I, I, I, P],
-    "friday_ops_rope_axes_kv_write": [P, T, T, P, P, P, P, PI, I, I, I, I, I, I, POINTER(KV), I, P],
+    "friday_ops_rotate_axes": [P, P, L, L, L, P, L, L, L, I, P, P, PI, I, I, I, I, I, P],
+    "friday_ops_rope_axes_kv_write": [P, P, L, L, L, P, L, L, L, I, P, P, P, P, PI, I, I, I, I, I, I, P, P, I, I, P, I, I, P],
     "friday_ops_attention_shared_floats": [P, I, I, I, I, I, I, I, I, I, I, I, POINTER(c_int64)],
-    "friday_ops_attention_shared": [P, T, c_int64, T, POINTER(KV), P, I, POINTER(Geometry), I, I, I, I, F, P, c_int64, P],
+    "friday_ops_attention_shared": [P, P, L, L, L, P, L, L, I, P, P, I, I, P, I, P, I, I, P, P, P, P, I, I, I, I, I, I, F, P, L, P],
     "friday_ops_sample": [P, T, P, P, P, c_uint64, P, P],
     "friday_ops_plan": [P, c_int64, c_int64, c_int64, PI, PI, PI],
     "friday_ops_decode_splits": [P, I, I, I, I, I, PI],
