@@ -17,6 +17,7 @@
 #include <stdlib.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -209,15 +210,343 @@ __global__ void __launch_bounds__(VEC == 4 ? 128 : 256) merge_kernel(const Share
     }
 }
 
-// ------------------------------------------------------------------ bf16 on the tensor cores
-// Both products are tcgen05.mma with scores, weights and results in tensor memory.  A tile is 128 rows of one kv head; row r of it
-// stands for (token row r / G, group head r % G), G = heads / kv heads.  For the prefix a tile's token rows are any consecutive rows
-// of the step, whatever sequences they belong to: that is what reads the prefix once for all.  For own keys they are rows of one
-// sequence.  A CTA has one tile and one of three jobs:
+// ------------------------------------------------------------------ jobs of tiles
+// Both kernels below work on tiles: the group heads of consecutive token rows, for one kv head.  For the prefix a tile's token rows are
+// any consecutive rows of the step, whatever sequences they belong to: that is what reads the prefix once for all.  For own keys they
+// are rows of one sequence.  A CTA has one tile and one of three jobs:
 //
-//   prefix   consecutive rows of the step, a share of the prefix' blocks            -> a part
+//   prefix   consecutive rows of the step, a share of the prefix' blocks of keys    -> a part
 //   own      rows of one sequence, a share of its own blocks                        -> a part
 //   whole    rows of one sequence, all of the prefix' blocks and then its own       -> the result (many rows per sequence)
+
+// a row's position, no further than the tables have room; -1: it sees nothing
+__device__ __forceinline__ int position_of(const SharedArgs& p, int row) {
+    const long long room = (long long)p.prefix + (long long)p.table_width * p.page;
+    return max(-1, (int)min((long long)p.row_pos[row], room - 1));
+}
+
+// Keys [lo, hi] of a range of pages that the CTA's rows see between them (none: hi < lo), block `first` its first one here, n blocks.
+struct Range {
+    int lo, hi, first, n;
+};
+struct Job {
+    int kvh, seq, row0, n_tok, part;      // n_tok token rows from row0 on
+    Range seg0, seg1;                     // of the prefix; of own keys, numbered from the prefix' end
+};
+
+// Tiles of one kv head and share of the prefix are neighbours in the grid: they read the same pages at about the same time.  CTAs start
+// in the order of their index: the prefix' shares (the most work) first, a whole job's late rows first.  T token rows make a tile;
+// s_pos: two numbers in shared memory, (INT_MAX, -1) behind a barrier.  For all threads of the block.
+__device__ __forceinline__ Job job_of(const SharedArgs& p, int T, int keys, int threads, int* s_pos) {
+    Job job;
+    const bool prefix_job = !p.whole && (int)blockIdx.x < p.prefix_ctas;
+    int share, shares;
+    if (prefix_job) {
+        const int per = p.prefix_ctas / (p.nkv * p.prefix_splits);
+        job.seq = 0;
+        job.row0 = blockIdx.x % per * T;
+        job.kvh = blockIdx.x / per % p.nkv;
+        share = blockIdx.x / (per * p.nkv);
+        shares = p.prefix_splits;
+        job.part = share;
+        job.n_tok = min(T, p.rows - job.row0);
+    } else {
+        const int x = blockIdx.x - p.prefix_ctas;
+        shares = p.whole ? 1 : p.own_splits;
+        const int per = (gridDim.x - p.prefix_ctas) / (p.n_seqs * p.nkv * shares);
+        job.seq = x % p.n_seqs;
+        job.kvh = x / p.n_seqs % p.nkv;
+        share = x / (p.n_seqs * p.nkv) % shares;
+        job.part = p.prefix_splits + share;
+        const int t0 = (per - 1 - x / (p.n_seqs * p.nkv * shares)) * T;
+        const int begin = p.seq_start[job.seq], count = begin < 0 || begin > p.rows ? 0 : min(p.seq_qlen[job.seq], p.rows - begin);
+        job.row0 = begin + t0;
+        job.n_tok = max(0, min(T, count - t0));
+    }
+    // Without a window a share of the prefix is the same whatever the rows' positions are.
+    job.seg0 = job.seg1 = Range{0, -1, 0, 0};
+    if (prefix_job && p.window == 0) {
+        job.seg0.hi = p.prefix - 1;
+    } else {
+        for (int t = threadIdx.x; t < job.n_tok; t += threads) {
+            const int of = p.row_seq[job.row0 + t];
+            if (of >= 0 && of < p.n_seqs) {
+                const int pos = position_of(p, job.row0 + t);
+                atomicMin(&s_pos[0], pos);
+                atomicMax(&s_pos[1], pos);
+            }
+        }
+        __syncthreads();
+        const int least = s_pos[0], most = s_pos[1];
+        const int lo = most < 0 ? 0 : fr_first_key(least, p.window, 0);
+        job.seg0.lo = lo;
+        job.seg1.lo = max(0, lo - p.prefix);
+        if (p.whole || prefix_job) job.seg0.hi = min(most, p.prefix - 1);
+        if (!prefix_job) job.seg1.hi = most - p.prefix;
+    }
+    auto take_share = [&](Range& g) {
+        if (g.hi < g.lo) return;
+        const int first = g.lo / keys, n = g.hi / keys - first + 1;
+        const int from = (int)((long long)n * share / shares), to = (int)((long long)n * (share + 1) / shares);
+        g.first = first + from;
+        g.n = to - from;
+    };
+    take_share(job.seg0);
+    take_share(job.seg1);
+    return job;
+}
+
+// ------------------------------------------------------------------ float32 in tiles
+// A block of 128 threads has 16 RPT rows and walks 32 keys at a time, which pass through shared memory once for all of them (two or
+// four stages, 16-byte asynchronous copies; what no row of the block sees, and pages that a table leaves out, come as zeros; the page
+// of a block is looked up a block before its copies are issued).  A thread has
+// the scores of up to RPT rows (4 of a warp side by side, 16 apart) with four keys, then the same rows' results in HD / 8 channels, so
+// that a row's scores, maximum and weights stay within a warp.  Bound by the multiply-adds where rows are many; a tile of few rows
+// (one token's group heads) only takes the 16-row steps that it has.
+namespace f32 {
+
+constexpr int KEYS = 32, THREADS = 128, LS = KEYS + 8;
+template <int HD>
+constexpr int stages() { return HD > 64 ? 2 : 4; }
+template <int HD, int RPT>
+constexpr int smem_bytes() { return (16 * RPT * (HD + 4) + stages<HD>() * KEYS * (2 * HD + 4) + 16 * RPT * LS) * 4; }
+
+template <int HD, int RPT>
+__global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
+    constexpr int ROWS = 16 * RPT, LQ = HD + 4, CH = HD / 32, STAGES = stages<HD>();      // CH: groups of four channels per thread
+    extern __shared__ __align__(16) float tile_smem[];
+    float* const sq = tile_smem;                                       // [ROWS][LQ]
+    float* const sk = sq + ROWS * LQ;                                  // [STAGES][KEYS][LQ]
+    float* const sv = sk + STAGES * KEYS * LQ;                         // [STAGES][KEYS][HD]
+    float* const sp = sv + STAGES * KEYS * HD;                         // [ROWS][LS]
+    __shared__ int s_pos[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ty = lane >> 3, tx = lane & 7;
+    if (tid == 0) {
+        s_pos[0] = 0x7fffffff;
+        s_pos[1] = -1;
+    }
+    __syncthreads();
+    fr_pdl_wait();
+    fr_pdl_launch();
+    const int G = p.nq / p.nkv, T = ROWS / G;
+    const Job job = job_of(p, T, KEYS, THREADS, s_pos);
+    const int n_rows = job.n_tok * G, n_blocks = job.seg0.n + job.seg1.n;
+    auto range_of = [&](int i, int& j0, bool& own) {
+        own = i >= job.seg0.n;
+        j0 = (own ? job.seg1.first + i - job.seg0.n : job.seg0.first + i) * KEYS;
+        return own ? job.seg1 : job.seg0;
+    };
+    // (pages that are whole blocks: all keys of a block lie in one)
+    const bool one_page = p.page % KEYS == 0;
+    auto page_of = [&](int i) {
+        if (!one_page || i >= n_blocks) return -1;
+        int j0;
+        bool own;
+        range_of(i, j0, own);
+        return own ? p.block_table[(size_t)job.seq * p.table_width + j0 / p.page] : p.prefix_table[j0 / p.page];
+    };
+    auto fetch = [&](int i, int page) {
+        if (i < n_blocks) {
+            int j0;
+            bool own;
+            const Range g = range_of(i, j0, own);
+            float* dk = sk + i % STAGES * KEYS * LQ;
+            float* dv = sv + i % STAGES * KEYS * HD;
+            const long long base = page >= 0 && page < p.pool_pages ? (long long)page * p.page + j0 % p.page : -1;
+#pragma unroll
+            for (int it = 0; it < KEYS * (HD / 4) / THREADS; ++it) {
+                const int idx = tid + it * THREADS, key = idx / (HD / 4), c = idx % (HD / 4) * 4, j = j0 + key;
+                long long at = -1;
+                if (j >= g.lo && j <= g.hi && c < p.hd) at = !one_page ? place_of(p, job.seq, own ? j + p.prefix : j) : base >= 0 ? base + key : -1;
+                const size_t from = at >= 0 ? ((size_t)at * p.nkv + job.kvh) * p.hd + c : 0;
+                const int bytes = at >= 0 ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dk + key * LQ + c)),
+                             "l"((const float*)p.k_pool + from), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dv + key * HD + c)),
+                             "l"((const float*)p.v_pool + from), "r"(bytes) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int ahead[STAGES - 1];
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) ahead[i] = page_of(i);
+    int next_page = page_of(STAGES - 1);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i, ahead[i]);
+    for (int idx = tid; idx < ROWS * (HD / 4); idx += THREADS) {
+        const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n_rows && c < p.hd) v = *(const float4*)((const float*)p.q + (size_t)(job.row0 + r / G) * p.q_stride + (size_t)(job.kvh * G + r % G) * p.hd + c);
+        v.x *= p.scale_log2; v.y *= p.scale_log2; v.z *= p.scale_log2; v.w *= p.scale_log2;
+        *(float4*)(sq + r * LQ + c) = v;
+    }
+    const int r0 = 4 * warp + ty;                                      // this thread's rows: r0 + 16 i
+    int pos[RPT], first[RPT];
+    bool live[RPT];
+    float m[RPT], l[RPT], acc[RPT][4 * CH];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int r = r0 + 16 * i;
+        live[i] = r < n_rows;
+        pos[i] = -1;
+        if (live[i]) {
+            const int of = p.row_seq[job.row0 + r / G];
+            live[i] = of >= 0 && of < p.n_seqs;
+            if (live[i]) pos[i] = position_of(p, job.row0 + r / G);
+        }
+        first[i] = fr_first_key(pos[i], p.window, 0);
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4 * CH; ++c) acc[i][c] = 0.f;
+    }
+    // one block of keys for the thread's first N rows
+    auto work = [&](auto number, int i) {
+        constexpr int N = decltype(number)::value;
+        int j0;
+        bool own;
+        range_of(i, j0, own);
+        const float* k0 = sk + i % STAGES * KEYS * LQ + tx * LQ;
+        float s[N][4];
+#pragma unroll
+        for (int a = 0; a < N; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) s[a][b] = 0.f;
+        // (sixteen dimensions at a time: the error of a score is that of short sums)
+#pragma unroll
+        for (int d0 = 0; d0 < HD; d0 += 16) {
+            float part[N][4];
+#pragma unroll
+            for (int a = 0; a < N; ++a)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) part[a][b] = 0.f;
+#pragma unroll
+            for (int d = d0; d < d0 + 16; d += 4) {
+                float4 q[N], k[4];
+#pragma unroll
+                for (int a = 0; a < N; ++a) q[a] = *(const float4*)(sq + (r0 + 16 * a) * LQ + d);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) k[b] = *(const float4*)(k0 + 8 * b * LQ + d);
+#pragma unroll
+                for (int a = 0; a < N; ++a)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        part[a][b] = fmaf(q[a].x, k[b].x, part[a][b]);
+                        part[a][b] = fmaf(q[a].y, k[b].y, part[a][b]);
+                        part[a][b] = fmaf(q[a].z, k[b].z, part[a][b]);
+                        part[a][b] = fmaf(q[a].w, k[b].w, part[a][b]);
+                    }
+            }
+#pragma unroll
+            for (int a = 0; a < N; ++a)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) s[a][b] += part[a][b];
+        }
+#pragma unroll
+        for (int a = 0; a < N; ++a) {
+            // columns hi < column or column < lo are masked
+            const int hi = (own ? pos[a] - p.prefix : min(pos[a], p.prefix - 1)) - j0, lo = first[a] - (own ? p.prefix : 0) - j0;
+            float big = m[a];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int key = tx + 8 * b;
+                if (key > hi || key < lo) s[a][b] = -INFINITY;
+                big = fmaxf(big, s[a][b]);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const float ref = big == -INFINITY ? 0.f : big;            // (nothing seen yet: weights against 0, all of them 0)
+            const float keep = exp2f(m[a] - ref);
+            float sum = 0.f;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float w = exp2f(s[a][b] - ref);
+                sum += w;
+                sp[(r0 + 16 * a) * LS + tx + 8 * b] = w;
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[a] = l[a] * keep + sum;
+            m[a] = big;
+#pragma unroll
+            for (int c = 0; c < 4 * CH; ++c) acc[a][c] *= keep;
+        }
+        __syncwarp();
+        const float* v0 = sv + i % STAGES * KEYS * HD + 4 * tx;
+#pragma unroll 2
+        for (int j = 0; j < KEYS; j += 4) {
+            float w[N][4];
+#pragma unroll
+            for (int a = 0; a < N; ++a) *(float4*)w[a] = *(const float4*)(sp + (r0 + 16 * a) * LS + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const float4 v = *(const float4*)(v0 + (j + e) * HD + 32 * c);
+#pragma unroll
+                    for (int a = 0; a < N; ++a) {
+                        acc[a][4 * c] = fmaf(w[a][e], v.x, acc[a][4 * c]);
+                        acc[a][4 * c + 1] = fmaf(w[a][e], v.y, acc[a][4 * c + 1]);
+                        acc[a][4 * c + 2] = fmaf(w[a][e], v.z, acc[a][4 * c + 2]);
+                        acc[a][4 * c + 3] = fmaf(w[a][e], v.w, acc[a][4 * c + 3]);
+                    }
+                }
+        }
+        __syncwarp();
+    };
+    const int steps = (n_rows - 4 * warp + 15) / 16;                   // 16-row steps in which this warp has rows
+    for (int i = 0; i < n_blocks; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncthreads();                                               // this block of keys is here, and everyone is done with the one before
+        fetch(i + STAGES - 1, next_page);
+        next_page = page_of(i + STAGES);
+        if (steps <= 0) continue;
+        if (RPT >= 2 && steps > RPT / 2) work(std::integral_constant<int, RPT>{}, i);
+        else if (RPT >= 4 && steps > RPT / 4) work(std::integral_constant<int, (RPT >= 2 ? RPT / 2 : 1)>{}, i);
+        else work(std::integral_constant<int, (RPT >= 4 ? RPT / 4 : 1)>{}, i);
+    }
+#pragma unroll
+    for (int a = 0; a < RPT; ++a) {
+        if (!live[a]) continue;
+        const int r = r0 + 16 * a;
+        const size_t item = (size_t)(job.row0 + r / G) * p.nq + (size_t)job.kvh * G + r % G, at = item * p.parts + job.part;
+        const float inv = l[a] > 0.f ? 1.f / l[a] : l[a];              // (nothing seen: 0; a NaN stays one)
+        float* to = p.whole ? (float*)p.out + item * p.hd : p.part + at * p.hd;
+        if (!p.whole && tx == 0) *(float2*)(p.stat + 2 * at) = make_float2(m[a], l[a]);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (4 * tx + 32 * c < p.hd)
+                *(float4*)(to + 4 * tx + 32 * c) = p.whole ? make_float4(acc[a][4 * c] * inv, acc[a][4 * c + 1] * inv, acc[a][4 * c + 2] * inv, acc[a][4 * c + 3] * inv)
+                                                           : make_float4(acc[a][4 * c], acc[a][4 * c + 1], acc[a][4 * c + 2], acc[a][4 * c + 3]);
+    }
+}
+
+template <int HD, int RPT>
+int launch(const SharedArgs& p, long long ctas, cudaStream_t stream) {
+    static std::atomic<unsigned long long> configured{0};             // a bit per device
+    int device = 0;
+    FR_CUDA(cudaGetDevice(&device));
+    const unsigned long long bit = 1ull << (device & 63);
+    if (!(configured.load() & bit)) {
+        FR_CUDA(cudaFuncSetAttribute(tiles_kernel<HD, RPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<HD, RPT>()));
+        configured.fetch_or(bit);
+    }
+    FR_CUDA(fr_launch(tiles_kernel<HD, RPT>, dim3((unsigned)ctas), dim3(THREADS), (size_t)smem_bytes<HD, RPT>(), stream, p));
+    FR_CHECK_LAUNCH("attention_shared (float32 tiles)");
+    return FR_OK;
+}
+
+template <int HD>
+int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t stream) {
+    return tile_rows == 64 ? launch<HD, 4>(p, ctas, stream) : tile_rows == 32 ? launch<HD, 2>(p, ctas, stream) : launch<HD, 1>(p, ctas, stream);
+}
+
+}  // namespace f32
+
+// ------------------------------------------------------------------ bf16 on the tensor cores
+// Both products are tcgen05.mma with scores, weights and results in tensor memory.  A tile is 128 rows of one kv head; row r of it
+// stands for (token row r / G, group head r % G), G = heads / kv heads.
 //
 //   warp 0      TMA: the queries (a 4-d box [64 dims][G heads][1][T rows] per 64-dim slice lands as rows t * G + g, 128-byte
 //               swizzle), then K of the block after and V of this one (a block of 64 keys is a page); a page that a table leaves out
@@ -313,17 +642,6 @@ __device__ __forceinline__ void mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_
         : "memory");
 }
 
-// a row's position, no further than the tables have room; -1: it sees nothing
-__device__ __forceinline__ int position_of(const SharedArgs& p, int row) {
-    const long long room = (long long)p.prefix + (long long)p.table_width * PAGE;
-    return max(-1, (int)min((long long)p.row_pos[row], room - 1));
-}
-
-// Keys [lo, hi] of a range of pages that the CTA's rows see between them (none: hi < lo), block `first` its first one here, n blocks.
-struct Range {
-    int lo, hi, first, n;
-};
-
 __global__ void __launch_bounds__(THREADS, 2)
 tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
              const SharedArgs p) {
@@ -370,63 +688,10 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     fr_pdl_wait();
     if (threadIdx.x == 0) fr_pdl_launch();
 
-    // The CTA's job.  Tiles of one kv head and share of the prefix are neighbours in the grid: they read the same pages at about the
-    // same time.  CTAs start in the order of their index: the prefix' shares (the most work) first, a whole job's late rows first.
     const int G = p.nq / p.nkv, T = ROWS / G;         // token rows of a tile
-    const bool prefix_job = !p.whole && (int)blockIdx.x < p.prefix_ctas;
-    int kvh, seq = 0, row0, n_tok, part, share, shares;
-    if (prefix_job) {
-        const int per = p.prefix_ctas / (p.nkv * p.prefix_splits);
-        row0 = blockIdx.x % per * T;
-        kvh = blockIdx.x / per % p.nkv;
-        share = blockIdx.x / (per * p.nkv);
-        shares = p.prefix_splits;
-        part = share;
-        n_tok = min(T, p.rows - row0);
-    } else {
-        const int x = blockIdx.x - p.prefix_ctas, splits = p.whole ? 1 : p.own_splits;
-        const int per = (gridDim.x - p.prefix_ctas) / (p.n_seqs * p.nkv * splits);
-        seq = x % p.n_seqs;
-        kvh = x / p.n_seqs % p.nkv;
-        share = x / (p.n_seqs * p.nkv) % splits;
-        shares = splits;
-        part = p.prefix_splits + share;
-        const int t0 = (per - 1 - x / (p.n_seqs * p.nkv * splits)) * T;
-        const int begin = p.seq_start[seq], count = begin < 0 || begin > p.rows ? 0 : min(p.seq_qlen[seq], p.rows - begin);
-        row0 = begin + t0;
-        n_tok = max(0, min(T, count - t0));
-    }
-    // Keys [lo, hi] that the CTA's rows see between them: of the prefix, of own ones (numbered from the prefix' end).  Without a window
-    // a share of the prefix is the same whatever the rows' positions are.
-    Range seg0{0, -1, 0, 0}, seg1{0, -1, 0, 0};
-    if (prefix_job && p.window == 0) {
-        seg0.hi = p.prefix - 1;
-    } else {
-        for (int t = threadIdx.x; t < n_tok; t += THREADS) {
-            const int of = p.row_seq[row0 + t];
-            if (of >= 0 && of < p.n_seqs) {
-                const int pos = position_of(p, row0 + t);
-                atomicMin(&s_pos[0], pos);
-                atomicMax(&s_pos[1], pos);
-            }
-        }
-        __syncthreads();
-        const int least = s_pos[0], most = s_pos[1];
-        const int lo = most < 0 ? 0 : fr_first_key(least, p.window, 0);
-        seg0.lo = lo;
-        seg1.lo = max(0, lo - p.prefix);
-        if (p.whole || prefix_job) seg0.hi = min(most, p.prefix - 1);
-        if (!prefix_job) seg1.hi = most - p.prefix;
-    }
-    auto take_share = [&](Range& g) {
-        if (g.hi < g.lo) return;
-        const int first = g.lo / KEYS, n = g.hi / KEYS - first + 1;
-        const int from = (int)((long long)n * share / shares), to = (int)((long long)n * (share + 1) / shares);
-        g.first = first + from;
-        g.n = to - from;
-    };
-    take_share(seg0);
-    take_share(seg1);
+    const Job job = job_of(p, T, KEYS, THREADS, s_pos);
+    const Range seg0 = job.seg0, seg1 = job.seg1;
+    const int kvh = job.kvh, seq = job.seq, row0 = job.row0, n_tok = job.n_tok, part = job.part;
     const int n_blocks = seg0.n + seg1.n;
     const int slices = (p.hd + 63) / 64;
     auto first_key_of = [&](int i) { return (i < seg0.n ? seg0.first + i : seg1.first + i - seg0.n) * KEYS; };
@@ -607,6 +872,10 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             const float inv = l_run > 0.f ? 1.f / l_run : l_run;
             const size_t at = item * p.parts + part;
             if (!p.whole && live) *(float2*)(p.stat + 2 * at) = make_float2(seen ? m_run : -INFINITY, l_run);
+            // A part's row leaves through shared memory (every product has read what lay there) as one bulk copy: 16-byte stores of 32
+            // lanes to 32 rows took 3.5 us a CTA, this BULK_TAIL.
+            const int pitch = p.hd * 4 + 16;                   // (eight lanes' pieces fall into different banks)
+            uint8_t* const line = smem + r * pitch;
 #pragma unroll 1
             for (int c = 0; c < p.hd; c += 16) {
                 uint32_t o16[16];
@@ -624,12 +893,17 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
                     *(uint4*)(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
                 } else if (seen) {
-                    float* dst = p.part + at * p.hd + c;
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4)
-                        *(float4*)(dst + j) = make_float4(__uint_as_float(o16[j]), __uint_as_float(o16[j + 1]), __uint_as_float(o16[j + 2]),
-                                                          __uint_as_float(o16[j + 3]));
+                    for (int j = 0; j < 16; j += 4) *(uint4*)(line + (c + j) * 4) = make_uint4(o16[j], o16[j + 1], o16[j + 2], o16[j + 3]);
                 }
+            }
+            if (!p.whole && live && seen) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.part + at * p.hd), "r"(smem_u32(line)),
+                             "r"((uint32_t)p.hd * 4)
+                             : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
         }
     }
@@ -686,7 +960,6 @@ int maps(const SharedArgs& p, CUtensorMap& mq, CUtensorMap& mk, CUtensorMap& mv)
 }
 
 int launch(const SharedArgs& p, long long ctas, cudaStream_t stream) {
-    if (ctas > 0x7fffffffLL) FR_REFUSE("attention_shared: %lld blocks exceed the grid", ctas);
     CUtensorMap mq, mk, mv;
     const int rc = maps(p, mq, mk, mv);
     if (rc) return rc;
@@ -726,33 +999,83 @@ Plan plan_rows(long long rows, int nq, int max_kv_len, int window) {
     return plan;
 }
 
-bool tiles_fit(int nq, int nkv, int hd, int page, int dtype) {
-    return dtype == FR_BF16 && hd % 16 == 0 && hd <= 128 && page == tcore::PAGE && nq / nkv <= tcore::ROWS;
+// What a tile is for a call: its rows and the keys of a block, how many CTAs an SM takes, and what they cost (us; measured): a CTA's
+// begin and end, a block of a full tile beside others (an SM's time over its CTAs) and alone, and one of the rows that a sequence has.
+struct TileKind {
+    int rows = 0, keys = 0, at_once = 0;                               // rows 0: no tiles for these sizes
+    double begin = 0, block = 0, alone = 0, own_block = 0, own_alone = 0;
+};
+
+TileKind kind_of(long long rows, int max_q_len, int nq, int nkv, int hd, int page, int dtype) {
+    TileKind k;
+    const int G = nq / nkv;
+    if (dtype == FR_BF16 && hd % 16 == 0 && hd <= 128 && page == tcore::PAGE && G <= tcore::ROWS) {
+        k.rows = tcore::ROWS;
+        k.keys = tcore::KEYS;
+        k.at_once = 2;
+        k.begin = 4.0; k.block = 0.95; k.alone = 0.85; k.own_block = 0.95; k.own_alone = 1.0;
+    } else if (dtype == FR_F32 && hd % 4 == 0 && hd <= 128 && G <= 64) {
+        const long long heads = rows * G;                              // rows that the prefix' tiles are made of
+        k.rows = heads > 32 || G > 32 ? 64 : heads > 16 || G > 16 ? 32 : 16;
+        k.keys = f32::KEYS;
+        k.at_once = hd <= 64 ? 3 : 2;
+        const long long own = (max_q_len < k.rows / G ? max_q_len : k.rows / G) * (long long)G;
+        const double steps = k.rows / 16, own_steps = own > 32 ? 4 : own > 16 ? 2 : 1, width = hd <= 32 ? 0.5 : hd <= 64 ? 1 : 2;
+        k.begin = 3.0; k.alone = width * (1.9 + 0.37 * steps); k.block = width * (1.0 + 1.2 * steps);
+        k.own_alone = width * (1.9 + 0.37 * own_steps); k.own_block = width * (1.0 + 1.2 * own_steps);
+    }
+    return k;
 }
 
-Plan plan_tiles(long long rows, int n_seqs, int max_q_len, int max_kv_len, int prefix, int nq, int nkv, int window) {
-    Plan plan;
+// How tiles share the work out, from an estimate of the time (us) of each way; a part of a row and head is written and read once.
+Plan plan_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_len, int max_kv_len, int prefix, int nq, int nkv, int hd, int window) {
+    const double begin = kind.begin, block = kind.block, part_us = hd * 3.6e-6;
     const int sms = fr_sm_count() > 0 ? fr_sm_count() : 148;
-    const int T = tcore::ROWS / (nq / nkv);
+    const int T = kind.rows / (nq / nkv);
     const long long all = (rows + T - 1) / T, own = (max_q_len + T - 1) / T;
-    int whole = 0, ps = -1, os = -1;
-    if (const char* e = getenv("FRIDAY_SHARED_PLAN")) sscanf(e, "%d,%d,%d", &whole, &ps, &os);
-    plan.tiles = (int)all;
-    plan.own_tiles = (int)own;
-    const long long slots = 2ll * sms, n_prefix = all * nkv, n_own = (long long)n_seqs * nkv * own;
+    const double slots = (double)kind.at_once * sms, tiles = (double)(n_seqs * own < all + n_seqs ? n_seqs * own : all + n_seqs);   // that sequences' rows make
     const long long prefix_reach = window > 0 && window < prefix ? window : prefix, own_reach = reach_of(max_kv_len - prefix, window);
-    const long long prefix_blocks = (prefix_reach + tcore::KEYS - 1) / tcore::KEYS, own_blocks = (own_reach + tcore::KEYS - 1) / tcore::KEYS;
-    if (whole) {
-        plan.whole = 1;
-        plan.ctas = n_own;
-        return plan;
+    const long long prefix_blocks = (prefix_reach + kind.keys - 1) / kind.keys, own_blocks = (own_reach + kind.keys - 1) / kind.keys;
+    Plan best;
+    best.tiles = (int)all;
+    best.own_tiles = (int)own;
+    // whole: every CTA walks everything
+    const double chain = (double)(prefix_blocks + own_blocks);
+    best.whole = 1;
+    best.ctas = (long long)n_seqs * nkv * own;
+    double least = begin + (tiles * nkv > slots ? (double)(long long)((tiles * nkv + slots - 1) / slots) * chain * block : chain * kind.own_alone);
+    static const int shares[] = {1, 2, 3, 4, 6, 8, 10, 12, 16, 20, 26, 32, 40, 48};
+    for (int os = 1; os <= 8; os *= 2) {
+        if (os > 1 && os > own_blocks) break;
+        for (int ps : shares) {
+            if (ps > 1 && ps > prefix_blocks) break;
+            const double p_chain = (double)((prefix_blocks + ps - 1) / ps), o_chain = (double)((own_blocks + os - 1) / os);
+            // (own sequences are half as long as the longest on average)
+            const double total = all * nkv * (ps * begin + prefix_blocks * block) + tiles * nkv * (os * begin + 0.5 * own_blocks * kind.own_block);
+            double us = total / slots;
+            if (us < begin + p_chain * kind.alone) us = begin + p_chain * kind.alone;
+            if (us < begin + o_chain * kind.own_alone) us = begin + o_chain * kind.own_alone;
+            us += 2.0 + rows * nq * (double)(ps + os) * part_us;
+            if (us < least) {
+                least = us;
+                best.whole = 0;
+                best.prefix_splits = ps;
+                best.own_splits = os;
+            }
+        }
     }
-    plan.prefix_splits = ps > 0 ? ps : clamp(slots / n_prefix, 1, clamp(prefix_blocks, 1, 40));
-    const long long each = (prefix_blocks + plan.prefix_splits - 1) / plan.prefix_splits;
-    plan.own_splits = os > 0 ? os : clamp(own_blocks / (each > 4 ? each : 4), 1, 16);
-    plan.parts = plan.prefix_splits + plan.own_splits;
-    plan.ctas = n_prefix * plan.prefix_splits + n_own * plan.own_splits;
-    return plan;
+    if (const char* e = getenv("FRIDAY_SHARED_PLAN")) {
+        best.prefix_splits = best.own_splits = 1;
+        sscanf(e, "%d,%d,%d", &best.whole, &best.prefix_splits, &best.own_splits);
+    }
+    if (!best.whole) {
+        best.parts = best.prefix_splits + best.own_splits;
+        best.ctas = all * nkv * best.prefix_splits + (long long)n_seqs * nkv * own * best.own_splits;
+    } else {
+        best.prefix_splits = best.own_splits = 0;
+        best.parts = 1;
+    }
+    return best;
 }
 
 long long floats_of(const Plan& plan, long long rows, int nq, int hd) { return plan.parts > 1 ? rows * nq * plan.parts * (hd + 2) + 1 : 0; }
@@ -774,8 +1097,9 @@ FR_EXPORT long long attention_shared_floats(int rows, int n_seqs, int max_q_len,
                                             int page, int window, int dtype) {
     if (rows <= 0 || n_seqs <= 0 || nq <= 0 || nkv <= 0 || nq < nkv || hd <= 0) return 0;
     const long long by_rows = floats_of(plan_rows(rows, nq, max_kv_len, window), rows, nq, hd);
-    if (!tiles_fit(nq, nkv, hd, page, dtype)) return by_rows;
-    const long long by_tiles = floats_of(plan_tiles(rows, n_seqs, max_q_len, max_kv_len, prefix, nq, nkv, window), rows, nq, hd);
+    const TileKind kind = kind_of(rows, max_q_len, nq, nkv, hd, page, dtype);
+    if (kind.rows == 0) return by_rows;
+    const long long by_tiles = floats_of(plan_tiles(kind, rows, n_seqs, max_q_len, max_kv_len, prefix, nq, nkv, hd, window), rows, nq, hd);
     return by_tiles > by_rows ? by_tiles : by_rows;
 }
 
@@ -799,11 +1123,12 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     p.row_seq = row_seq; p.row_pos = row_pos; p.q_stride = q_stride; p.rows = rows; p.n_seqs = n_seqs; p.nq = nq; p.nkv = nkv; p.hd = hd;
     p.window = window; p.prefix = prefix; p.page = page; p.pool_pages = pool_pages; p.table_width = table_width;
     p.scale_log2 = scale * 1.4426950408889634f; p.seq_start = seq_start; p.seq_qlen = seq_qlen; p.status = status;
-    // TMA wants rows that start on 16-byte boundaries, and row numbers of 32 bits
-    const bool tiles = tiles_fit(nq, nkv, hd, page, dtype) && q_stride % 8 == 0 &&
+    // Copies of 16 bytes want rows that start on 16-byte boundaries, TMA row numbers of 32 bits.
+    const TileKind kind = kind_of(rows, max_q_len, nq, nkv, hd, page, dtype);
+    const bool tiles = kind.rows > 0 && q_stride % (dtype == FR_BF16 ? 8 : 4) == 0 &&
                        (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0 &&
                        pool_pages < 0x7fffffff / tcore::PAGE && status != nullptr;
-    const Plan plan = tiles ? plan_tiles(rows, n_seqs, max_q_len, max_kv_len, prefix, nq, nkv, window) : plan_rows(rows, nq, max_kv_len, window);
+    const Plan plan = tiles ? plan_tiles(kind, rows, n_seqs, max_q_len, max_kv_len, prefix, nq, nkv, hd, window) : plan_rows(rows, nq, max_kv_len, window);
     if (scratch_floats < floats_of(plan, rows, nq, hd)) FR_REFUSE("attention_shared: %lld floats of working memory are too few", scratch_floats);
     p.parts = plan.parts;
     p.part = scratch;
@@ -811,8 +1136,12 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     if (tiles) {
         p.whole = plan.whole; p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits;
         p.prefix_ctas = plan.whole ? 0 : plan.tiles * nkv * plan.prefix_splits;
-        p.covered = plan.own_tiles * (tcore::ROWS / (nq / nkv));
-        const int rc = tcore::launch(p, plan.ctas, stream);
+        p.covered = plan.own_tiles * (kind.rows / (nq / nkv));
+        if (plan.ctas > 0x7fffffffLL) FR_REFUSE("attention_shared: %lld blocks exceed the grid", plan.ctas);
+        const int rc = dtype == FR_BF16 ? tcore::launch(p, plan.ctas, stream)
+                       : hd <= 32       ? f32::launch_rows<32>(p, kind.rows, plan.ctas, stream)
+                       : hd <= 64       ? f32::launch_rows<64>(p, kind.rows, plan.ctas, stream)
+                                        : f32::launch_rows<128>(p, kind.rows, plan.ctas, stream);
         if (rc != FR_OK) return rc;
     } else {
         const int rc = dtype == FR_F32 ? launch_rows<float>(p, stream) : launch_rows<bf16>(p, stream);
