@@ -49,7 +49,7 @@ struct SharedArgs {
     const int* seq_qlen;
     int* status;
     int whole;                // 1: a CTA walks prefix and own keys of one sequence's rows; 0: CTAs of one or the other, parts joined
-    int prefix_ctas, prefix_splits, own_splits;           // prefix_splits 0: parts are not of one range or the other
+    int jobs, prefix_jobs, prefix_splits, own_splits;           // prefix_splits 0: parts are not of one range or the other
     int covered;              // rows of a sequence that the grid's own tiles reach
 };
 
@@ -153,9 +153,16 @@ __global__ void __launch_bounds__(VEC == 4 ? 128 : 256) merge_kernel(const Share
             else to[0] = from[(size_t)s * p.hd];
         }
     };
+    // lane s has the statistics of parts s and s + 32
+    float2 ml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
+    if (tid < 32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (lane + 32 * i < p.parts) ml[i] = *(const float2*)(p.stat + 2 * ((size_t)item * p.parts + lane + 32 * i));
+    }
+    const int seq = p.row_seq[row];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) fetch(sub + i * at_once, v[i]);
-    const int seq = p.row_seq[row];
     if (seq < 0 || seq >= p.n_seqs) return;
     if (tid < 32) {
         // own parts are there for rows that the sequence's range names
@@ -164,15 +171,11 @@ __global__ void __launch_bounds__(VEC == 4 ? 128 : 256) merge_kernel(const Share
             const int t = row - p.seq_start[seq];
             if (t < 0 || t >= min(p.seq_qlen[seq], p.covered)) parts = p.prefix_splits;
         }
-        // lane s has the statistics of parts s and s + 32
-        const float* stat = p.stat + 2 * (size_t)item * p.parts;
         float m[2], l[2], f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const bool there = lane + 32 * i < parts;
-            const float2 ml = there ? *(const float2*)(stat + 2 * (lane + 32 * i)) : make_float2(-INFINITY, 0.f);
-            l[i] = ml.y;
-            m[i] = l[i] == 0.f ? -INFINITY : ml.x;
+            l[i] = lane + 32 * i < parts ? ml[i].y : 0.f;
+            m[i] = l[i] == 0.f ? -INFINITY : ml[i].x;
         }
         const float big = fr_warp_max(fmaxf(m[0], m[1]));
 #pragma unroll
@@ -234,29 +237,54 @@ struct Job {
     Range seg0, seg1;                     // of the prefix; of own keys, numbered from the prefix' end
 };
 
-// Tiles of one kv head and share of the prefix are neighbours in the grid: they read the same pages at about the same time.  CTAs start
-// in the order of their index: the prefix' shares (the most work) first, a whole job's late rows first.  T token rows make a tile;
-// s_pos: two numbers in shared memory, (INT_MAX, -1) behind a barrier.  For all threads of the block.
-__device__ __forceinline__ Job job_of(const SharedArgs& p, int T, int keys, int threads, int* s_pos) {
+// The sequences by their last position, greatest first (ties: the lower number first): own jobs are taken longest first.
+__device__ __forceinline__ void order_by_length(const SharedArgs& p, int* s_order, int* s_last) {
+    int last = -1;
+    const int s = threadIdx.x;
+    if (s < p.n_seqs) {
+        const int begin = p.seq_start[s], count = p.seq_qlen[s];
+        if (count > 0 && begin >= 0 && begin + (long long)count <= p.rows) last = p.row_pos[begin + count - 1];
+        s_last[s] = last;
+    }
+    __syncthreads();
+    if (s < p.n_seqs) {
+        int before = 0;
+        for (int other = 0; other < p.n_seqs; ++other) {
+            const int theirs = s_last[other];
+            before += theirs > last || (theirs == last && other < s) ? 1 : 0;
+        }
+        s_order[before] = s;
+    }
+    __syncthreads();
+}
+
+// Job number `index` of p.jobs.  Tiles of one kv head and share of the prefix are neighbours: they read the same pages at about the same
+// time.  The prefix' shares (the most work) come first, a whole job's late rows first.  T token rows make a tile; s_pos: two numbers in
+// shared memory, (INT_MAX, -1) behind a barrier; s_order: the sequences in the order in which they are taken (null: their own).  For all
+// threads of the block.
+__device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int keys, int threads, int* s_pos, const int* s_order) {
     Job job;
-    const bool prefix_job = !p.whole && (int)blockIdx.x < p.prefix_ctas;
+    const bool prefix_job = !p.whole && index < p.prefix_jobs;
     int share, shares;
     if (prefix_job) {
-        const int per = p.prefix_ctas / (p.nkv * p.prefix_splits);
+        const int per = p.prefix_jobs / (p.nkv * p.prefix_splits);
         job.seq = 0;
-        job.row0 = blockIdx.x % per * T;
-        job.kvh = blockIdx.x / per % p.nkv;
-        share = blockIdx.x / (per * p.nkv);
+        job.row0 = index % per * T;
+        job.kvh = index / per % p.nkv;
+        share = index / (per * p.nkv);
         shares = p.prefix_splits;
         job.part = share;
         job.n_tok = min(T, p.rows - job.row0);
     } else {
-        const int x = blockIdx.x - p.prefix_ctas;
+        const int x = index - p.prefix_jobs;
         shares = p.whole ? 1 : p.own_splits;
-        const int per = (gridDim.x - p.prefix_ctas) / (p.n_seqs * p.nkv * shares);
-        job.seq = x % p.n_seqs;
-        job.kvh = x / p.n_seqs % p.nkv;
-        share = x / (p.n_seqs * p.nkv) % shares;
+        const int per = (p.jobs - p.prefix_jobs) / (p.n_seqs * p.nkv * shares);
+        // (whole: the sequences' tiles of one rank together; else the shares and kv heads of a sequence)
+        const int inner = p.whole ? p.n_seqs : p.nkv * shares;
+        const int s = p.whole ? x % inner : x / inner % p.n_seqs, rest = p.whole ? x / inner % p.nkv : x % inner;
+        job.seq = s_order != nullptr ? s_order[s] : s;
+        job.kvh = rest % p.nkv;
+        share = rest / p.nkv;
         job.part = p.prefix_splits + share;
         const int t0 = (per - 1 - x / (p.n_seqs * p.nkv * shares)) * T;
         const int begin = p.seq_start[job.seq], count = begin < 0 || begin > p.rows ? 0 : min(p.seq_qlen[job.seq], p.rows - begin);
@@ -329,7 +357,7 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
     fr_pdl_wait();
     fr_pdl_launch();
     const int G = p.nq / p.nkv, T = ROWS / G;
-    const Job job = job_of(p, T, KEYS, THREADS, s_pos);
+    const Job job = job_of(p, (int)blockIdx.x, T, KEYS, THREADS, s_pos, nullptr);
     const int n_rows = job.n_tok * G, n_blocks = job.seg0.n + job.seg1.n;
     auto range_of = [&](int i, int& j0, bool& own) {
         own = i >= job.seg0.n;
@@ -573,7 +601,7 @@ constexpr int SLICE = ROWS * 128;         // bytes of 128 rows of 64 numbers
 constexpr int KEYS = 64, THREADS = 192;
 constexpr int KSLICE = KEYS * 128, STAGE = 2 * KSLICE;        // a block's keys (or values): two slices of 64 dims
 constexpr int TMEM = 256;                                     // columns: S of even blocks, S of odd blocks (P over each one's first half), O
-constexpr int SMEM = 2 * SLICE + 4 * STAGE + 1024 + 256;
+constexpr int SMEM = 2 * SLICE + 4 * STAGE + 1024 + 256 + 2 * 4 * THREADS;      // (256: barriers and single words)
 
 __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -653,7 +681,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     uint64_t* bars = (uint64_t*)(s_v + 2 * STAGE);
     // bars: q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2]
     uint32_t* tmem_slot = (uint32_t*)(bars + 15);
-    int* s_pos = (int*)(tmem_slot + 1);               // least, greatest position of a live row
+    int* s_pos = (int*)(tmem_slot + 1);               // least, greatest position of a live row; a wait gave up; then room for order_by_length
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t q_full = smem_u32(bars), k_full = smem_u32(bars + 1), k_empty = smem_u32(bars + 3);
@@ -673,6 +701,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         s_pos[0] = 0x7fffffff;
         s_pos[1] = -1;
+        s_pos[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -689,21 +718,35 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (threadIdx.x == 0) fr_pdl_launch();
 
     const int G = p.nq / p.nkv, T = ROWS / G;         // token rows of a tile
-    const Job job = job_of(p, T, KEYS, THREADS, s_pos);
+    const int slices = (p.hd + 63) / 64;
+    int* s_order = nullptr;
+    if (!p.whole && p.n_seqs <= THREADS && p.jobs > (int)gridDim.x) {
+        s_order = s_pos + 3;
+        order_by_length(p, s_order, s_order + THREADS);
+    }
+    // The CTA's jobs: one of every round of the grid, each round in the other direction than the one before, so that who had the
+    // longest of a round has the shortest of the next.
+    int blocks_before = 0, loads_before = 0;          // blocks and queries' tiles of the jobs so far: what the barriers' phases count
+    for (int round = 0;; ++round) {
+    const long long index = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    if ((long long)round * gridDim.x >= p.jobs) break;
+    if (index >= p.jobs) continue;
+    const Job job = job_of(p, (int)index, T, KEYS, THREADS, s_pos, s_order);
     const Range seg0 = job.seg0, seg1 = job.seg1;
     const int kvh = job.kvh, seq = job.seq, row0 = job.row0, n_tok = job.n_tok, part = job.part;
-    const int n_blocks = seg0.n + seg1.n;
-    const int slices = (p.hd + 63) / 64;
+    const int n_blocks = seg0.n + seg1.n, before = blocks_before;
     auto first_key_of = [&](int i) { return (i < seg0.n ? seg0.first + i : seg1.first + i - seg0.n) * KEYS; };
     auto last_key_of = [&](int i) { return i < seg0.n ? seg0.hi : seg1.hi; };
+    // stage of block i, and the parity of that stage's use
+    auto stage_of = [&](int i) { return (before + i) & 1; };
+    auto parity_of = [&](int i) { return ((before + i) >> 1) & 1; };
 
-    // Block i uses stage i & 1 of K, V and S, in their (i >> 1)-th use.
     if (warp == 0) {
         if (n_blocks > 0 && elect_one()) {
             mbar_expect_tx(q_full, (uint32_t)(slices * 64 * G * T * 2));
             for (int s = 0; s < slices; ++s) load_4d(smem_u32(s_q + s * SLICE), &map_q, s * 64, 0, kvh, row0, q_full);
             auto load = [&](int i, const CUtensorMap* map, uint8_t* ring, uint32_t full, uint32_t empty) {
-                const int b = i & 1, par = (i >> 1) & 1;
+                const int b = stage_of(i), par = parity_of(i);
                 if (!mbar_wait(empty + 8 * b, par ^ 1, p.status, 1)) return false;
                 mbar_expect_tx(full + 8 * b, (uint32_t)(slices * KSLICE));
                 const int* table = i < seg0.n ? p.prefix_table : p.block_table + (size_t)seq * p.table_width;
@@ -718,17 +761,18 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 if (i + 1 < n_blocks) ok = load(i + 1, &map_k, s_k, k_full, k_empty);
                 if (ok) ok = load(i, &map_v, s_v, v_full, v_empty);
             }
+            if (!ok) s_pos[2] = 1;
         }
     } else if (warp == 1) {
         if (n_blocks > 0 && elect_one()) {
             const uint32_t idesc_qk = instr_desc(ROWS, KEYS);
             const uint32_t idesc_pv = instr_desc(ROWS, p.hd) | (1u << 16);              // B is MN-major
             const int k_steps = p.hd / 16;
-            bool ok = mbar_wait(q_full, 0, p.status, 2);
+            bool ok = mbar_wait(q_full, loads_before & 1, p.status, 2);
             // (descriptors are made once and stepped: a lone thread issues all of this)
             const uint64_t dq0 = smem_desc(smem_u32(s_q)), dk0 = smem_desc(smem_u32(s_k)), dv0 = desc_mn(smem_u32(s_v), KSLICE, 1024);
             auto scores = [&](int i) {
-                const int b = i & 1, par = (i >> 1) & 1;
+                const int b = stage_of(i), par = parity_of(i);
                 if (!mbar_wait(k_full + 8 * b, par, p.status, 3)) return false;
                 tc_fence_after();
                 uint64_t da = dq0, db = dk0 + (uint64_t)(b * (STAGE >> 4));
@@ -748,7 +792,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             if (ok) ok = scores(0);
             if (ok && n_blocks > 1) ok = scores(1);
             for (int i = 0; i < n_blocks && ok; ++i) {
-                const int b = i & 1, par = (i >> 1) & 1;
+                const int b = stage_of(i), par = parity_of(i);
                 if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 4))) break;
                 if (!(ok = mbar_wait(p_full + 8 * b, par, p.status, 5))) break;
                 tc_fence_after();
@@ -765,6 +809,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 tc_commit(v_empty + 8 * b);
                 if (i + 2 < n_blocks) ok = scores(i + 2);
             }
+            if (!ok) s_pos[2] = 1;
         }
     } else {
         const int quarter = warp & 3;                          // the tensor-memory lanes that this warp may touch: 32 * quarter ..
@@ -783,7 +828,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
         for (int i = 0; i < n_blocks; ++i) {
-            const int b = i & 1, par = (i >> 1) & 1;
+            const int b = stage_of(i), par = parity_of(i);
             const bool own = i >= seg0.n;
             const int j0 = first_key_of(i);
             if (!(ok = mbar_wait(s_full + 8 * b, par, p.status, 6))) break;
@@ -816,7 +861,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     if (i > 0) {
                         // Every product into O so far must be done: that of block i - 2 is (this block's scores were issued behind
                         // it), so the wait for the other stage's phase is unambiguous.
-                        if (!(ok = mbar_wait(pv_done + 8 * (b ^ 1), ((i - 1) >> 1) & 1, p.status, 8))) break;
+                        if (!(ok = mbar_wait(pv_done + 8 * (b ^ 1), parity_of(i - 1), p.status, 8))) break;
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < p.hd; c += 16) {
@@ -863,9 +908,10 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             mbar_arrive(p_full + 8 * b);
         }
         if (ok && n_blocks > 0) {
-            ok = mbar_wait(pv_done + 8 * ((n_blocks - 1) & 1), ((n_blocks - 1) >> 1) & 1, p.status, 8);
+            ok = mbar_wait(pv_done + 8 * stage_of(n_blocks - 1), parity_of(n_blocks - 1), p.status, 8);
             tc_fence_after();
         }
+        if (!ok) s_pos[2] = 1;
         if (ok && any) {
             const size_t item = (size_t)row * p.nq + (size_t)kvh * G + g;
             const bool seen = l_run != 0.f;                    // (a NaN is seen)
@@ -907,12 +953,20 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             }
         }
     }
+    // the job's products, copies and reads are done for all roles
+    blocks_before += n_blocks;
+    loads_before += n_blocks > 0 ? 1 : 0;
+    if (threadIdx.x == 0) {
+        s_pos[0] = 0x7fffffff;
+        s_pos[1] = -1;
+    }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM) : "memory");
+    tc_fence_after();
+    if (s_pos[2] != 0) break;                         // (the phases are no longer known)
     }
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM) : "memory");
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -959,7 +1013,7 @@ int maps(const SharedArgs& p, CUtensorMap& mq, CUtensorMap& mk, CUtensorMap& mv)
     return FR_OK;
 }
 
-int launch(const SharedArgs& p, long long ctas, cudaStream_t stream) {
+int launch(const SharedArgs& p, long long jobs, cudaStream_t stream) {
     CUtensorMap mq, mk, mv;
     const int rc = maps(p, mq, mk, mv);
     if (rc) return rc;
@@ -971,7 +1025,9 @@ int launch(const SharedArgs& p, long long ctas, cudaStream_t stream) {
         FR_CUDA(cudaFuncSetAttribute(tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         configured.fetch_or(bit);
     }
-    FR_CUDA(fr_launch(tiles_kernel, dim3((unsigned)ctas), dim3(THREADS), SMEM, stream, mq, mk, mv, p));
+    const long long most = 2ll * (fr_sm_count() > 0 ? fr_sm_count() : 148);
+    // (whole jobs, many of which a ragged batch does not have, are dealt out as CTAs end)
+    FR_CUDA(fr_launch(tiles_kernel, dim3((unsigned)(jobs < most || p.whole ? jobs : most)), dim3(THREADS), SMEM, stream, mq, mk, mv, p));
     FR_CHECK_LAUNCH("attention_shared (tiles)");
     return FR_OK;
 }
@@ -1043,17 +1099,20 @@ Plan plan_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_len,
     const double chain = (double)(prefix_blocks + own_blocks);
     best.whole = 1;
     best.ctas = (long long)n_seqs * nkv * own;
-    double least = begin + (tiles * nkv > slots ? (double)(long long)((tiles * nkv + slots - 1) / slots) * chain * block : chain * kind.own_alone);
-    static const int shares[] = {1, 2, 3, 4, 6, 8, 10, 12, 16, 20, 26, 32, 40, 48};
+    double least = begin + (tiles * nkv > slots ? (double)(long long)((tiles * nkv + slots - 1) / slots) * chain * block : chain * kind.alone);
+    // (one of them: as many as leave every SM one share)
+    const int shares[] = {1, 2, 3, 4, 6, 8, 10, 12, 16, 20, 26, 32, 40, clamp(sms / (all * nkv), 1, 40), clamp(prefix_blocks, 1, MOST_PARTS - 8)};
     for (int os = 1; os <= 8; os *= 2) {
         if (os > 1 && os > own_blocks) break;
         for (int ps : shares) {
-            if (ps > 1 && ps > prefix_blocks) break;
+            if (ps > 1 && ps > prefix_blocks) continue;
             const double p_chain = (double)((prefix_blocks + ps - 1) / ps), o_chain = (double)((own_blocks + os - 1) / os);
             // (own sequences are half as long as the longest on average)
             const double total = all * nkv * (ps * begin + prefix_blocks * block) + tiles * nkv * (os * begin + 0.5 * own_blocks * kind.own_block);
             double us = total / slots;
-            if (us < begin + p_chain * kind.alone) us = begin + p_chain * kind.alone;
+            // (a share of the prefix beside another one on its SM, or beside own keys only)
+            const double p_block = all * nkv * ps > sms ? block : kind.alone;
+            if (us < begin + p_chain * p_block) us = begin + p_chain * p_block;
             if (us < begin + o_chain * kind.own_alone) us = begin + o_chain * kind.own_alone;
             us += 2.0 + rows * nq * (double)(ps + os) * part_us;
             if (us < least) {
@@ -1134,10 +1193,11 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     p.part = scratch;
     p.stat = scratch + ((long long)rows * nq * plan.parts * hd + 1) / 2 * 2;           // (pairs of numbers)
     if (tiles) {
+        if (plan.ctas > 0x7fffffffLL) FR_REFUSE("attention_shared: %lld jobs are too many", plan.ctas);
         p.whole = plan.whole; p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits;
-        p.prefix_ctas = plan.whole ? 0 : plan.tiles * nkv * plan.prefix_splits;
+        p.jobs = (int)plan.ctas;
+        p.prefix_jobs = plan.whole ? 0 : plan.tiles * nkv * plan.prefix_splits;
         p.covered = plan.own_tiles * (kind.rows / (nq / nkv));
-        if (plan.ctas > 0x7fffffffLL) FR_REFUSE("attention_shared: %lld blocks exceed the grid", plan.ctas);
         const int rc = dtype == FR_BF16 ? tcore::launch(p, plan.ctas, stream)
                        : hd <= 32       ? f32::launch_rows<32>(p, kind.rows, plan.ctas, stream)
                        : hd <= 64       ? f32::launch_rows<64>(p, kind.rows, plan.ctas, stream)
