@@ -14,7 +14,7 @@
 #include <cuda.h>
 #include <math.h>
 
-#include <stdlib.h>
+#include <string.h>
 
 #include <atomic>
 #include <type_traits>
@@ -631,17 +631,6 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
-        "%25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -660,6 +649,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// the greatest of three; two sums, two multiply-adds in one instruction
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long two(float lo, float hi) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void halves(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 // D[tmem] (+)= A[tmem] * B[smem]: lane = row, two bf16 per column of A
 __device__ __forceinline__ void mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -849,8 +860,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 // (the maximum in four strands; the positive scale is applied to the result)
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < KEYS; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(raw[j]));
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+                for (int j = 0; j < KEYS; j += 2) mx4[(j >> 1) & 3] = max3(mx4[(j >> 1) & 3], __uint_as_float(raw[j]), __uint_as_float(raw[j + 1]));
+                const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * p.scale_log2;
                 const bool grow = mx > m_run + 8.f;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float alpha = grow ? exp2f(m_run - mx) : 1.f;      // 0 for a row that had seen no key
@@ -877,19 +888,26 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 }
                 // a masked score is -inf and stays so; a row that has seen no key takes its exponentials against 0
                 const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-                float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t packed[KEYS / 2];
+                const unsigned long long scale2 = two(p.scale_log2, p.scale_log2), neg2 = two(neg_m, neg_m);
+                unsigned long long sum2[2] = {0ull, 0ull};
 #pragma unroll
-                for (int j = 0; j < KEYS; j += 2) {
-                    const float e0 = exp2_fast(fmaf(__uint_as_float(raw[j]), p.scale_log2, neg_m));
-                    const float e1 = exp2_fast(fmaf(__uint_as_float(raw[j + 1]), p.scale_log2, neg_m));
-                    sum4[j & 2] += e0;
-                    sum4[(j & 2) + 1] += e1;
-                    packed[j >> 1] = pack2(e0, e1);
+                for (int h = 0; h < 2; ++h) {                  // (a half is on its way while the other is made)
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float x0, x1;
+                        halves(fma2(two(__uint_as_float(raw[32 * h + j]), __uint_as_float(raw[32 * h + j + 1])), scale2, neg2), x0, x1);
+                        const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
+                        sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], two(e0, e1));
+                        packed[j >> 1] = pack2(e0, e1);
+                    }
+                    st16(t_s + 16 * h, packed);
                 }
-                st32(t_s, packed);
-                st_wait();
+                float sum4[4];
+                halves(sum2[0], sum4[0], sum4[1]);
+                halves(sum2[1], sum4[2], sum4[3]);
                 l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+                st_wait();
             }
             const int in_lo = (own ? seg1.lo : seg0.lo) - j0, in_hi = last_key_of(i) - j0;
             if (in_lo > 0 || in_hi < KEYS - 1) {
@@ -1084,7 +1102,7 @@ TileKind kind_of(long long rows, int max_q_len, int nq, int nkv, int hd, int pag
 }
 
 // How tiles share the work out, from an estimate of the time (us) of each way; a part of a row and head is written and read once.
-Plan plan_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_len, int max_kv_len, int prefix, int nq, int nkv, int hd, int window) {
+Plan estimate_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_len, int max_kv_len, int prefix, int nq, int nkv, int hd, int window) {
     const double begin = kind.begin, block = kind.block, part_us = hd * 3.6e-6;
     const int sms = fr_sm_count() > 0 ? fr_sm_count() : 148;
     const int T = kind.rows / (nq / nkv);
@@ -1123,10 +1141,6 @@ Plan plan_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_len,
             }
         }
     }
-    if (const char* e = getenv("FRIDAY_SHARED_PLAN")) {
-        best.prefix_splits = best.own_splits = 1;
-        sscanf(e, "%d,%d,%d", &best.whole, &best.prefix_splits, &best.own_splits);
-    }
     if (!best.whole) {
         best.parts = best.prefix_splits + best.own_splits;
         best.ctas = all * nkv * best.prefix_splits + (long long)n_seqs * nkv * own * best.own_splits;
@@ -1135,6 +1149,18 @@ Plan plan_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_len,
         best.parts = 1;
     }
     return best;
+}
+
+// The same for the sizes that came before: a step's layers ask for the same way again and again.
+Plan plan_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_len, int max_kv_len, int prefix, int nq, int nkv, int hd, int window) {
+    const long long sizes[] = {kind.rows, kind.keys, rows, n_seqs, max_q_len, max_kv_len, prefix, nq, nkv, hd, window};
+    static thread_local long long known[sizeof sizes / sizeof sizes[0]] = {};
+    static thread_local Plan plan;
+    if (memcmp(known, sizes, sizeof sizes) != 0) {
+        plan = estimate_tiles(kind, rows, n_seqs, max_q_len, max_kv_len, prefix, nq, nkv, hd, window);
+        memcpy(known, sizes, sizeof sizes);
+    }
+    return plan;
 }
 
 long long floats_of(const Plan& plan, long long rows, int nq, int hd) { return plan.parts > 1 ? rows * nq * plan.parts * (hd + 2) + 1 : 0; }

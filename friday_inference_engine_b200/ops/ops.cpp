@@ -1820,9 +1820,10 @@ void Ops::attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const
     q_rows.shape[0] = rows;
     if (rows_collide(q_rows, n, out, n, false)) throw KernelError("attention_shared: the result overlaps the queries");
     const auto& k = kernels::attention_shared();
-    const int64_t floats = attention_shared_floats(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, view.page_size, window, out.dtype);
-    if (place && place->scratch_floats < floats) throw KernelError(format("attention_shared: %lld floats of scratch are needed", (long long)floats));
-    float* scratch = floats == 0 ? nullptr : place ? place->scratch : scratch_floats(floats);
+    // (a caller's scratch that is too small is refused by the launcher)
+    const int64_t floats = place ? place->scratch_floats
+                                 : attention_shared_floats(rows, ctx.n_seqs, ctx.max_q_len, ctx.max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, view.page_size, window, out.dtype);
+    float* scratch = place ? place->scratch : floats > 0 ? scratch_floats(floats) : nullptr;
     std::unique_ptr<Timed> t(place ? nullptr : new Timed(*this, Attention));
     int launches = 0;
     const int rc = k.run(q.data, q_stride, out.data, view.k_pool, view.v_pool, view.pool_pages, view.page_size, prefix_table, prefix_len, view.block_table,
