@@ -8,8 +8,7 @@ ordered with the torch operations around them.  (rotate_axes, rope_axes_kv_write
 attention_shared run on torch's current stream instead, may be captured into a CUDA graph
 there, and may be called from several threads at once.)
 """
-from ctypes import byref, c_int, c_int64, c_void_p
-from functools import lru_cache
+from ctypes import byref, c_int, c_void_p
 
 from .. import native
 
@@ -55,40 +54,29 @@ def _ref(struct):
     return None if struct is None else byref(struct)
 
 
-_ROW_CODES = None
+def _torch_ops():
+    """The extension module that takes torch tensors (binding/torch_ops.cpp), built on first use."""
+    global _torch_ops
+    import importlib.machinery
+    import importlib.util
+    from ctypes import cast
 
+    import torch  # noqa: F401 - its libraries have to be loaded first
 
-def _row_codes():
-    """dtypes of rows -> the kernels' numbers for them"""
-    global _ROW_CODES
-    if _ROW_CODES is None:
-        import torch
-        _ROW_CODES = {torch.float32: 0, torch.bfloat16: 1}
-    return _ROW_CODES
-
-
-def _current_stream(device):
-    global _current_stream
-    import torch
-    _current_stream = torch._C._cuda_getCurrentRawStream
-    return _current_stream(device)
-
-
-@lru_cache(maxsize=256)
-def _sections_of(values):
-    import torch
-    s = tuple(map(int, values))
-    if not 1 <= len(s) <= 4 or min(s) < 0 or sum(s) < 1:
-        raise ValueError
-    return (c_int * len(s))(*s), len(s), sum(s), torch.int32, torch.float32
-
-
-def _sections(sections):
-    """(host array, number of sections, pairs in all, and the dtypes of positions and denominators)"""
+    from . import build
     try:
-        return _sections_of(tuple(sections))
-    except (TypeError, ValueError):
-        raise native.KernelError("1 to 4 sections (pairs per axis) with at least one pair between them are wanted, got %r" % (sections,)) from None
+        path = build.ensure_binding_built()
+    except build.BuildError as e:
+        raise native.BuildError(str(e)) from None
+    loader = importlib.machinery.ExtensionFileLoader("friday_torch_ops", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("friday_torch_ops", path, loader=loader))
+    loader.exec_module(module)
+    library = native.lib()
+    module.init(*(cast(getattr(library, "friday_ops_" + name), c_void_p).value
+                  for name in ("rotate_axes", "rope_axes_kv_write", "attention_shared", "attention_shared_floats")), native.check,
+                native.KernelError)
+    _torch_ops = lambda: module          # noqa: E731 - from here on the module itself
+    return module
 
 
 class DeferredNorm:
@@ -137,7 +125,6 @@ class CudaOps:
 
     def __init__(self, device=0):
         self.device = int(device)
-        self._floats_of = {}                       # attention_shared: floats of scratch by a call's sizes
         self._h = c_void_p()
         native.call("friday_ops_new", int(device), None, byref(self._h))
 
@@ -288,63 +275,16 @@ class CudaOps:
         return s.value
 
     # -- a batch that shares a long prefix, positions with several axes ----
-    # These run on torch's current stream; what a call needs of scratch is torch's, so that a captured graph has its own.  A step of a
-    # few rows is over in the time of some thirty Python calls: every check is part of one condition, and what is wrong is looked for
-    # only once that fails.
-    def _rows_wrong(self, what, **tensors):
-        for name, t in tensors.items():
-            if t.get_device() != self.device:
-                raise native.KernelError("%s: %s is on %s, these operations are cuda:%d's" % (what, name, t.device, self.device))
-            if t.dtype not in _row_codes() or t.dim() != 2:
-                raise native.KernelError("%s: %s must be rows of float32 or bfloat16, got %s %s" % (what, name, t.dtype, tuple(t.shape)))
-            if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-                raise native.KernelError("%s: %s needs unit inner stride and rows apart, got strides %s" % (what, name, t.stride()))
-
-    def _numbers_wrong(self, what, **arrays):
-        import torch
-        for name, (t, shape) in arrays.items():
-            whole = isinstance(shape, tuple)
-            if (t.dtype != torch.int32 or t.get_device() != self.device or not t.is_contiguous() or (tuple(t.shape) != shape if whole else t.numel() < shape)):
-                raise native.KernelError("%s: %s must be %s contiguous int32 numbers on cuda:%d, got %s %s with strides %s on %s"
-                                         % (what, name, list(shape) if whole else "at least %d" % shape, self.device, t.dtype, tuple(t.shape),
-                                            t.stride(), t.device))
-
-    def _axes_wrong(self, what, rows, positions, denom, axes, pairs):
-        self._numbers_wrong(what, positions=(positions, (rows, axes)))
-        raise native.KernelError("%s: denom must be %d contiguous float32 numbers on cuda:%d, one per pair, got %s %s on %s"
-                                 % (what, pairs, self.device, denom.dtype, tuple(denom.shape), denom.device))
-
-    def _cache_wrong(self, what, k_pool, v_pool, block_table, shape):
-        self._numbers_wrong(what, block_table=(block_table, 0))
-        if block_table.dim() != 2:
-            raise native.KernelError("%s: the block table is [sequences, pages], got %s" % (what, tuple(block_table.shape)))
-        raise native.KernelError("%s: keys and values need pools of their own, contiguous [pages, %d, %d, %d] of float32 or bfloat16 on cuda:%d, "
-                                 "got %s %s and %s %s" % ((what,) + shape + (self.device, k_pool.dtype, tuple(k_pool.shape), v_pool.dtype, tuple(v_pool.shape))))
-
+    # These run on torch's current stream; results and scratch are torch's, so that a captured graph has its own.  Arguments are
+    # checked in binding/torch_ops.cpp.
     def rotate_axes(self, x, positions, denom, sections, heads, head_dim, interleaved=False, neighbours=False, out=None):
         """The first `heads` heads of every row of x [rows, >= heads * head_dim], turned: pair i of a head by
         positions[row][axis of i] / denom[i].  sections: pairs per axis (time, height, width; up to 4), one axis after another, or
         with `interleaved` in turn: pair i belongs to axis i mod n if i < n * sections[i mod n], else to axis 0.  A pair is
         (i, i + pairs), with `neighbours` (2i, 2i + 1); dimensions behind the pairs stay.  out [rows, heads * head_dim] may be x's own
         columns (None: a new tensor).  positions int32 [rows, axes], denom float32 [pairs], not zero.  -> out"""
-        array, axes, pairs, i32, f32 = _sections(sections)
-        if out is None:
-            out = x.new_empty((x.shape[0], max(int(heads), 0) * max(int(head_dim), 0)))
-        device, codes, shape, at, to, place = self.device, _row_codes(), x.shape, x.stride(), out.stride(), out.shape
-        if not (x.get_device() == device == out.get_device() and x.dtype in codes and out.dtype is x.dtype and len(shape) == 2 == len(place)
-                and (at[1] == 1 or shape[1] < 2) and (to[1] == 1 or place[1] < 2) and (shape[0] < 2 or (at[0] >= shape[1] and to[0] >= place[1]))):
-            self._rows_wrong("rotate_axes", x=x, out=out)
-            raise native.KernelError("rotate_axes: x and out are of one dtype, got %s and %s" % (x.dtype, out.dtype))
-        rows = shape[0]
-        if not (positions.dtype is i32 and positions.shape == (rows, axes) and positions.get_device() == device == denom.get_device()
-                and positions.is_contiguous() and denom.dtype is f32 and denom.numel() == pairs and denom.is_contiguous()):
-            self._axes_wrong("rotate_axes", rows, positions, denom, axes, pairs)
-        if rows == 0:
-            return out
-        native.check(native.lib().friday_ops_rotate_axes(
-            self._h, x.data_ptr(), rows, shape[1], at[0], out.data_ptr(), place[0], place[1], to[0], codes[x.dtype], positions.data_ptr(),
-            denom.data_ptr(), array, axes, interleaved, neighbours, heads, head_dim, _current_stream(device)))
-        return out
+        return _torch_ops().rotate_axes(self._h.value, self.device, x, heads, head_dim, positions, denom, sections, interleaved,
+                                        neighbours, out)
 
     def rope_axes_kv_write(self, qkv, row_seq, row_pos, positions, denom, sections, n_heads, n_kv_heads, head_dim, k_pool, v_pool,
                            block_table, page_size, interleaved=False, neighbours=False, q_out=None):
@@ -353,43 +293,8 @@ class CudaOps:
         page block_table[row_seq][row_pos / page_size], row row_pos mod page_size.  Nothing else of qkv changes.  Rows whose row_seq
         is negative are left alone; a row whose place the table does not name only gets its queries.  No two rows of a call may name
         the same place.  -> q_out"""
-        what = "rope_axes_kv_write"
-        array, axes, pairs, i32, f32 = _sections(sections)
-        if q_out is None:
-            q_out = qkv.new_empty((qkv.shape[0], max(int(n_heads), 0) * max(int(head_dim), 0)))
-        device, codes, shape, at, to, place = self.device, _row_codes(), qkv.shape, qkv.stride(), q_out.stride(), q_out.shape
-        if not (qkv.get_device() == device == q_out.get_device() and qkv.dtype in codes and q_out.dtype is qkv.dtype and len(shape) == 2 == len(place)
-                and (at[1] == 1 or shape[1] < 2) and (to[1] == 1 or place[1] < 2) and (shape[0] < 2 or (at[0] >= shape[1] and to[0] >= place[1]))):
-            self._rows_wrong(what, qkv=qkv, q_out=q_out)
-            raise native.KernelError("%s: qkv and q_out are of one dtype, got %s and %s" % (what, qkv.dtype, q_out.dtype))
-        rows = shape[0]
-        if not (positions.dtype is i32 and positions.shape == (rows, axes) and positions.get_device() == device == denom.get_device()
-                and positions.is_contiguous() and denom.dtype is f32 and denom.numel() == pairs and denom.is_contiguous()):
-            self._axes_wrong(what, rows, positions, denom, axes, pairs)
-        if not (row_seq.dtype is i32 and row_pos.dtype is i32 and row_seq.get_device() == device == row_pos.get_device() and row_seq.is_contiguous()
-                and row_pos.is_contiguous() and row_seq.numel() >= rows and row_pos.numel() >= rows):
-            self._numbers_wrong(what, row_seq=(row_seq, rows), row_pos=(row_pos, rows))
-        k, v, pages, table, seqs, width = self._cache(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim)
-        if k_pool.dtype is not qkv.dtype:
-            raise native.KernelError("%s: the cache's dtype differs from the rows'" % what)
-        if rows == 0 or seqs == 0:
-            return q_out
-        if width == 0:
-            raise native.KernelError("%s: the block table is empty" % what)
-        native.check(native.lib().friday_ops_rope_axes_kv_write(
-            self._h, qkv.data_ptr(), rows, shape[1], at[0], q_out.data_ptr() if n_heads > 0 else None, place[0], place[1], to[0], codes[qkv.dtype],
-            row_seq.data_ptr(), row_pos.data_ptr(), positions.data_ptr(), denom.data_ptr(), array, axes, interleaved, neighbours, n_heads,
-            n_kv_heads, head_dim, k, v, pages, page_size, table, seqs, width, _current_stream(device)))
-        return q_out
-
-    def _cache(self, what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim):
-        shape, device, dtype, k, v = k_pool.shape, self.device, k_pool.dtype, k_pool.data_ptr(), v_pool.data_ptr()
-        table = block_table.shape
-        if not (dtype in _row_codes() and v_pool.dtype is dtype and v_pool.shape == shape and len(shape) == 4 and shape[1:] == (page_size, n_kv_heads, head_dim)
-                and shape[0] > 0 and k != v and k_pool.is_contiguous() and v_pool.is_contiguous() and k_pool.get_device() == device == v_pool.get_device()
-                and _codes().get(block_table.dtype) == 2 and len(table) == 2 and block_table.is_contiguous() and block_table.get_device() == device):
-            self._cache_wrong(what, k_pool, v_pool, block_table, (page_size, n_kv_heads, head_dim))
-        return k, v, shape[0], block_table.data_ptr(), table[0], table[1]
+        return _torch_ops().rope_axes_kv_write(self._h.value, self.device, qkv, n_heads, n_kv_heads, head_dim, positions, denom, sections,
+                                               interleaved, neighbours, row_seq, row_pos, k_pool, v_pool, block_table, page_size, q_out)
 
     def attention_shared(self, q, q_stride, out, k_pool, v_pool, prefix_table, prefix_len, block_table, page_size, row_seq, row_pos,
                          n_heads, n_kv_heads, head_dim, window, scale, geometry):
@@ -404,54 +309,9 @@ class CudaOps:
         device): the rows of sequence s are seq_start[s] and the seq_qlen[s] - 1 after it, row_seq says so too.  max_q_len bounds
         seq_qlen; max_kv_len is a bound on the positions that only shares the work out.  prefix_len is a number of the host's: a
         captured graph keeps it."""
-        what = "attention_shared"
-        device, codes, shape, at, to, place = self.device, _row_codes(), q.shape, q.stride(), out.stride(), out.shape
-        if not (q.get_device() == device == out.get_device() and q.dtype in codes and out.dtype is q.dtype and len(shape) == 2 == len(place)
-                and (at[1] == 1 or shape[1] < 2) and (to[1] == 1 or place[1] < 2) and (shape[0] < 2 or (at[0] >= shape[1] and at[0] == q_stride))
-                and (place[0] < 2 or to[0] == place[1])):
-            self._rows_wrong(what, q=q, out=out)
-            raise native.KernelError("%s: queries and results of one dtype, queries q_stride apart and results contiguous are wanted, got %s with strides %s, "
-                                     "q_stride %s, and %s with strides %s" % (what, q.dtype, at, q_stride, out.dtype, to))
-        rows, window, prefix_len = place[0], int(window or 0), int(prefix_len)
-        k, v, pages, table, seqs, width = self._cache(what, k_pool, v_pool, block_table, page_size, n_kv_heads, head_dim)
-        if k_pool.dtype is not q.dtype:
-            raise native.KernelError("%s: the cache's dtype differs from the queries'" % what)
-        n_seqs, max_q_len, max_kv_len, starts, lens = geometry.n_seqs, geometry.max_q_len, geometry.max_kv_len, geometry.seq_start, geometry.seq_qlen
-        i32 = row_seq.dtype
-        if not (i32 is block_table.dtype and row_pos.dtype is i32 and starts.dtype is i32 and lens.dtype is i32
-                and row_seq.get_device() == row_pos.get_device() == starts.get_device() == lens.get_device() == device
-                and row_seq.is_contiguous() and row_pos.is_contiguous() and starts.is_contiguous() and lens.is_contiguous()
-                and row_seq.numel() >= rows and row_pos.numel() >= rows and starts.numel() >= n_seqs and lens.numel() >= n_seqs):
-            self._numbers_wrong(what, row_seq=(row_seq, rows), row_pos=(row_pos, rows), seq_start=(starts, n_seqs), seq_qlen=(lens, n_seqs))
-        if seqs < n_seqs:
-            raise native.KernelError("%s: %d sequences, a block table of %d" % (what, n_seqs, seqs))
-        prefix = None
-        if prefix_len > 0:
-            if prefix_table is None:
-                raise native.KernelError("%s: a prefix of %d needs its pages" % (what, prefix_len))
-            if not (prefix_table.dtype is i32 and prefix_table.get_device() == device and prefix_table.is_contiguous()
-                    and prefix_table.numel() * page_size >= prefix_len):
-                self._numbers_wrong(what, prefix_table=(prefix_table, -(-prefix_len // page_size)))
-            prefix = prefix_table.data_ptr()
-        if rows == 0 or n_seqs <= 0:
-            return
-        code = codes[q.dtype]
-        floats = self._shared_floats(rows, n_seqs, max_q_len, max_kv_len, prefix_len, n_heads, n_kv_heads, head_dim, page_size, window, code)
-        scratch = q.new_empty(floats * (4 // q.element_size())) if floats else None
-        native.check(native.lib().friday_ops_attention_shared(
-            self._h, q.data_ptr(), shape[0], shape[1], q_stride, out.data_ptr(), rows, place[1], code, k, v, pages, page_size, prefix, prefix_len,
-            table, n_seqs, width, row_seq.data_ptr(), row_pos.data_ptr(), starts.data_ptr(), lens.data_ptr(), max_q_len, max_kv_len, n_heads,
-            n_kv_heads, head_dim, window, scale, scratch.data_ptr() if floats else None, floats, _current_stream(device)))
-
-    def _shared_floats(self, *sizes):
-        got = self._floats_of.get(sizes)
-        if got is None:
-            n = c_int64()
-            native.call("friday_ops_attention_shared_floats", self._h, *sizes, byref(n))
-            if len(self._floats_of) >= 4096:                  # (sizes of a step: a few of them come again and again)
-                self._floats_of.clear()
-            got = self._floats_of[sizes] = n.value
-        return got
+        _torch_ops().attention_shared(self._h.value, self.device, q, q_stride, out, n_heads, n_kv_heads, head_dim, k_pool, v_pool, block_table,
+                                      page_size, prefix_table, prefix_len, row_seq, row_pos, window, scale, geometry.n_seqs,
+                                      geometry.max_q_len, geometry.max_kv_len, geometry.seq_start, geometry.seq_qlen)
 
     # -- one attention kernel's launcher, called directly with chosen arguments (tests of that kernel alone) -----
     def _test_buffers(self, device):

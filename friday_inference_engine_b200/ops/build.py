@@ -15,6 +15,9 @@ per-user folder under the system's temporary directory.
 
     python -m friday_inference_engine_b200.ops.build        # everything, for C++ users
 
+One file more is for Python alone: binding/torch_ops.cpp becomes friday_torch_ops.so, an extension module made against the
+installed torch (the operators whose calls must cost little).
+
 There is no fallback: a library that cannot be built or loaded raises.
 """
 import hashlib
@@ -276,11 +279,74 @@ def ensure_engine_built(progress=True):
     return engine_library_path()
 
 
+# ---------------------------------------------------------------------------------------
+# the extension module that takes torch tensors
+# ---------------------------------------------------------------------------------------
+
+BINDING = os.path.join(PACKAGE, "binding", "torch_ops.cpp")
+
+
+def binding_path():
+    return os.path.join(build_dir(), "friday_torch_ops.so")
+
+
+BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w"]
+_binding_lock = threading.Lock()
+
+
+def _binding_command(out):
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cmd = [_cxx()] + BINDING_FLAGS + ["-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I", INCLUDE]
+    for folder in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                   os.path.join(_cuda_home(), "include"), sysconfig.get_paths()["include"]):
+        cmd += ["-isystem", folder]
+    libs = os.path.join(root, "lib")
+    return cmd + ["-o", out, BINDING, "-L", libs, "-Wl,-rpath," + libs, "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+
+
+def _binding_fingerprint():
+    import torch
+    h = hashlib.sha1()
+    for d in (BINDING, os.path.join(INCLUDE, "friday", "capi.h")):
+        with open(d, "rb") as f:
+            h.update(f.read() + b"\0")
+    h.update(("%s %s %s %s" % (torch.__version__, os.path.dirname(torch.__file__), sys.version, " ".join(BINDING_FLAGS))).encode())
+    return h.hexdigest()
+
+
+def ensure_binding_built(progress=True):
+    """Compiles binding/torch_ops.cpp unless the module was made from the present source, for this torch and this Python."""
+    with _binding_lock:
+        lib, want = binding_path(), _binding_fingerprint()
+        try:
+            with open(lib + ".sha1") as f:
+                if os.path.exists(lib) and f.read().strip() == want:
+                    return lib
+        except OSError:
+            pass
+        t0 = time.time()
+        if progress:
+            print("[friday] compiling the binding for torch tensors", file=sys.stderr, flush=True)
+        tmp = "%s.%d.tmp" % (lib, os.getpid())
+        cmd = _binding_command(tmp)
+        proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if proc.returncode != 0:
+            raise BuildError("the C++ compiler failed for %s:\n%s\n%s" % (BINDING, " ".join(cmd), proc.stdout))
+        os.replace(tmp, lib)
+        with open(lib + ".sha1", "w") as f:
+            f.write(want)
+        if progress:
+            print("[friday] binding built in %.0f s" % (time.time() - t0), file=sys.stderr, flush=True)
+        return lib
+
+
 def build_all(progress=True):
     fams = [f for f in FAMILIES if os.path.exists(os.path.join(CSRC, f + ".cu"))]
     engine = ensure_engine_built(progress=progress)
     ensure_built(fams, progress=progress)
-    return [engine] + [library_path(f) for f in fams]
+    return [engine] + [library_path(f) for f in fams] + [ensure_binding_built(progress=progress)]
 
 
 if __name__ == "__main__":
