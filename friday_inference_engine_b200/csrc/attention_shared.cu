@@ -235,6 +235,7 @@ struct Range {
 struct Job {
     int kvh, seq, row0, n_tok, part;      // n_tok token rows from row0 on
     Range seg0, seg1;                     // of the prefix; of own keys, numbered from the prefix' end
+    bool early;
 };
 
 // The sequences by their last position, greatest first (ties: the lower number first): own jobs are taken longest first.
@@ -261,8 +262,9 @@ __device__ __forceinline__ void order_by_length(const SharedArgs& p, int* s_orde
 // Job number `index` of p.jobs.  Tiles of one kv head and share of the prefix are neighbours: they read the same pages at about the same
 // time.  The prefix' shares (the most work) come first, a whole job's late rows first.  T token rows make a tile; s_pos: two numbers in
 // shared memory, (INT_MAX, -1) behind a barrier; s_order: the sequences in the order in which they are taken (null: their own).  For all
-// threads of the block.
-__device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int keys, int threads, int* s_pos, const int* s_order) {
+// threads of the block.  early: a share of the prefix without a window does not wait for the rows' positions; its range then ends with
+// the prefix, wherever the last of its rows is.
+__device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int keys, int threads, int* s_pos, const int* s_order, bool early) {
     Job job;
     const bool prefix_job = !p.whole && index < p.prefix_jobs;
     int share, shares;
@@ -291,9 +293,9 @@ __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int
         job.row0 = begin + t0;
         job.n_tok = max(0, min(T, count - t0));
     }
-    // Without a window a share of the prefix is the same whatever the rows' positions are.
     job.seg0 = job.seg1 = Range{0, -1, 0, 0};
-    if (prefix_job && p.window == 0) {
+    job.early = early && prefix_job && p.window == 0;
+    if (job.early) {
         job.seg0.hi = p.prefix - 1;
     } else {
         for (int t = threadIdx.x; t < job.n_tok; t += threads) {
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
     fr_pdl_wait();
     fr_pdl_launch();
     const int G = p.nq / p.nkv, T = ROWS / G;
-    const Job job = job_of(p, (int)blockIdx.x, T, KEYS, THREADS, s_pos, nullptr);
+    const Job job = job_of(p, (int)blockIdx.x, T, KEYS, THREADS, s_pos, nullptr, false);
     const int n_rows = job.n_tok * G, n_blocks = job.seg0.n + job.seg1.n;
     auto range_of = [&](int i, int& j0, bool& own) {
         own = i >= job.seg0.n;
@@ -692,7 +694,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     uint64_t* bars = (uint64_t*)(s_v + 2 * STAGE);
     // bars: q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2]
     uint32_t* tmem_slot = (uint32_t*)(bars + 15);
-    int* s_pos = (int*)(tmem_slot + 1);               // least, greatest position of a live row; a wait gave up; then room for order_by_length
+    int* s_pos = (int*)(tmem_slot + 1);               // a wait gave up; least, greatest position of a live row, for even and odd rounds; then room for order_by_length
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t q_full = smem_u32(bars), k_full = smem_u32(bars + 1), k_empty = smem_u32(bars + 3);
@@ -710,9 +712,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             mbar_init(p_full + 8 * b, 128);
             mbar_init(pv_done + 8 * b, 1);
         }
-        s_pos[0] = 0x7fffffff;
-        s_pos[1] = -1;
-        s_pos[2] = 0;
+        s_pos[0] = 0;
+        s_pos[1] = s_pos[3] = 0x7fffffff;
+        s_pos[2] = s_pos[4] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -732,7 +734,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     const int slices = (p.hd + 63) / 64;
     int* s_order = nullptr;
     if (!p.whole && p.n_seqs <= THREADS && p.jobs > (int)gridDim.x) {
-        s_order = s_pos + 3;
+        s_order = s_pos + 5;
         order_by_length(p, s_order, s_order + THREADS);
     }
     // The CTA's jobs: one of every round of the grid, each round in the other direction than the one before, so that who had the
@@ -742,7 +744,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     const long long index = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     if ((long long)round * gridDim.x >= p.jobs) break;
     if (index >= p.jobs) continue;
-    const Job job = job_of(p, (int)index, T, KEYS, THREADS, s_pos, s_order);
+    int* const s_range = s_pos + 1 + 2 * (round & 1);
+    const Job job = job_of(p, (int)index, T, KEYS, THREADS, s_range, s_order, true);
     const Range seg0 = job.seg0, seg1 = job.seg1;
     const int kvh = job.kvh, seq = job.seq, row0 = job.row0, n_tok = job.n_tok, part = job.part;
     const int n_blocks = seg0.n + seg1.n, before = blocks_before;
@@ -772,7 +775,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 if (i + 1 < n_blocks) ok = load(i + 1, &map_k, s_k, k_full, k_empty);
                 if (ok) ok = load(i, &map_v, s_v, v_full, v_empty);
             }
-            if (!ok) s_pos[2] = 1;
+            if (!ok) s_pos[0] = 1;
         }
     } else if (warp == 1) {
         if (n_blocks > 0 && elect_one()) {
@@ -820,7 +823,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 tc_commit(v_empty + 8 * b);
                 if (i + 2 < n_blocks) ok = scores(i + 2);
             }
-            if (!ok) s_pos[2] = 1;
+            if (!ok) s_pos[0] = 1;
         }
     } else {
         const int quarter = warp & 3;                          // the tensor-memory lanes that this warp may touch: 32 * quarter ..
@@ -835,6 +838,12 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         const int first = fr_first_key(pos, p.window, 0);
         const bool any = __any_sync(0xffffffffu, live);        // a warp without rows only keeps the barriers going
+        int prefix_hi = seg0.hi;                               // the last prefix position that a row of the CTA sees
+        if (job.early) {
+            if (live) atomicMax(&s_range[1], pos);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            prefix_hi = min(seg0.hi, s_range[1]);
+        }
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16, t_o = tmem + lane_addr + 2 * KEYS;
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
@@ -909,7 +918,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
                 st_wait();
             }
-            const int in_lo = (own ? seg1.lo : seg0.lo) - j0, in_hi = last_key_of(i) - j0;
+            const int in_lo = (own ? seg1.lo : seg0.lo) - j0, in_hi = (own ? seg1.hi : prefix_hi) - j0;
             if (in_lo > 0 || in_hi < KEYS - 1) {
                 // positions that no row of the CTA sees: their values may be anything
                 if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 7))) break;
@@ -929,7 +938,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             ok = mbar_wait(pv_done + 8 * stage_of(n_blocks - 1), parity_of(n_blocks - 1), p.status, 8);
             tc_fence_after();
         }
-        if (!ok) s_pos[2] = 1;
+        if (!ok) s_pos[0] = 1;
         if (ok && any) {
             const size_t item = (size_t)row * p.nq + (size_t)kvh * G + g;
             const bool seen = l_run != 0.f;                    // (a NaN is seen)
@@ -975,13 +984,14 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     blocks_before += n_blocks;
     loads_before += n_blocks > 0 ? 1 : 0;
     if (threadIdx.x == 0) {
-        s_pos[0] = 0x7fffffff;
-        s_pos[1] = -1;
+        // the next round's pair of positions, which nobody has read since the round before this one
+        s_pos[1 + 2 * (round + 1 & 1)] = 0x7fffffff;
+        s_pos[2 + 2 * (round + 1 & 1)] = -1;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (s_pos[2] != 0) break;                         // (the phases are no longer known)
+    if (s_pos[0] != 0) break;                         // (the phases are no longer known)
     }
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM) : "memory");
@@ -1015,7 +1025,6 @@ int maps(const SharedArgs& p, CUtensorMap& mq, CUtensorMap& mk, CUtensorMap& mv)
     const int G = p.nq / p.nkv;
     {
         const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)G, (cuuint64_t)p.nkv, (cuuint64_t)p.rows};
-        // (the stride between rows of a lone row is never used, but has to be one that a map takes)
         const cuuint64_t strides[3] = {(cuuint64_t)p.hd * 2, (cuuint64_t)G * p.hd * 2, (cuuint64_t)p.q_stride * 2};
         const cuuint32_t box[4] = {64, (cuuint32_t)G, 1, (cuuint32_t)(ROWS / G)};
         const int rc = encode(&mq, p.q, 4, dims, strides, box, "the queries");
@@ -1060,7 +1069,7 @@ struct Plan {
 };
 
 // Keys a row may see in all, at most.
-long long reach_of(int max_kv_len, int window) { return window > 0 && window < max_kv_len ? window : max_kv_len; }
+long long reach_of(long long max_kv_len, int window) { return window > 0 && window < max_kv_len ? window : max_kv_len; }
 
 int clamp(long long v, long long lo, long long hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
 
@@ -1108,7 +1117,7 @@ Plan estimate_tiles(const TileKind& kind, long long rows, int n_seqs, int max_q_
     const int T = kind.rows / (nq / nkv);
     const long long all = (rows + T - 1) / T, own = (max_q_len + T - 1) / T;
     const double slots = (double)kind.at_once * sms, tiles = (double)(n_seqs * own < all + n_seqs ? n_seqs * own : all + n_seqs);   // that sequences' rows make
-    const long long prefix_reach = window > 0 && window < prefix ? window : prefix, own_reach = reach_of(max_kv_len - prefix, window);
+    const long long prefix_reach = window > 0 && window < prefix ? window : prefix, own_reach = reach_of(max_kv_len > prefix ? max_kv_len - prefix : 0, window);
     const long long prefix_blocks = (prefix_reach + kind.keys - 1) / kind.keys, own_blocks = (own_reach + kind.keys - 1) / kind.keys;
     Plan best;
     best.tiles = (int)all;
@@ -1203,6 +1212,7 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     if (prefix < 0 || page < 1 || pool_pages < 1 || table_width < 0 || window < 0)
         FR_REFUSE("attention_shared: prefix %d, pages of %d, %d of them, a table %d wide, window %d", prefix, page, pool_pages, table_width, window);
     if (!(scale > 0.f) || !(scale < INFINITY)) FR_REFUSE("attention_shared: a scale of %g", (double)scale);
+    if (rows == 1) q_stride = (long long)nq * hd;                      // (of a lone row it is never used)
     SharedArgs p = {};
     p.q = q; p.out = out; p.k_pool = k_pool; p.v_pool = v_pool; p.prefix_table = prefix_table; p.block_table = block_table;
     p.row_seq = row_seq; p.row_pos = row_pos; p.q_stride = q_stride; p.rows = rows; p.n_seqs = n_seqs; p.nq = nq; p.nkv = nkv; p.hd = hd;

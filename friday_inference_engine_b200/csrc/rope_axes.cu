@@ -401,10 +401,8 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
 
 int check(const RopeArgs& p, int dtype, const int* sections) {
     if (dtype != FR_F32 && dtype != FR_BF16) FR_REFUSE("rope_axes: unknown dtype %d", dtype);
-    if (p.axes < 1 || p.axes > MOST_AXES) FR_REFUSE("rope_axes: %d axes (1 to %d)", p.axes, MOST_AXES);
     if (p.hd < 1 || p.nq < 0 || p.nkv < 0 || p.nq + p.nkv < 1) FR_REFUSE("rope_axes: %d heads, %d kv heads of %d numbers", p.nq, p.nkv, p.hd);
-    for (int a = 0; a < p.axes; ++a)
-        if (sections[a] < 0 || sections[a] > MOST_HALF) FR_REFUSE("rope_axes: a section of %d pairs", sections[a]);
+    if ((long long)(p.nq + 2ll * p.nkv) * p.hd > 0x3fffffffLL) FR_REFUSE("rope_axes: rows of %lld numbers", (long long)(p.nq + 2ll * p.nkv) * p.hd);
     if (p.half < 1 || p.half > MOST_HALF || 2 * p.half > p.hd)
         FR_REFUSE("rope_axes: sections of %d pairs in all do not fit heads of %d numbers (and %d pairs are the most)", p.half, p.hd, MOST_HALF);
     if (p.interleaved)
@@ -515,8 +513,10 @@ cudaError_t launch_rows(const RopeArgs& p, cudaStream_t stream) {
 }
 
 int launch(RopeArgs& p, const int* sections, int dtype, cudaStream_t stream) {
+    if (p.axes < 1 || p.axes > MOST_AXES) FR_REFUSE("rope_axes: %d axes (1 to %d)", p.axes, MOST_AXES);
     p.half = 0;
-    for (int a = 0; a < p.axes && a < MOST_AXES; ++a) {
+    for (int a = 0; a < p.axes; ++a) {
+        if (sections[a] < 0 || sections[a] > MOST_HALF) FR_REFUSE("rope_axes: a section of %d pairs", sections[a]);
         p.half += sections[a];
         p.section_end[a] = p.interleaved ? sections[a] : p.half;
     }

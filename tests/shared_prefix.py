@@ -47,15 +47,16 @@ class Batch:
     no sequence holds, and the rows behind a sequence's end, are NaN."""
 
     def __init__(self, dtype, q_lens, own_lens, prefix, heads, kv_heads, hd, window=0, seed=0, device="cuda:0", spread=1.5, beside=0,
-                 wider=0, pool_extra=3):
+                 wider=0, pool_extra=3, page=PAGE):
         g = torch.Generator().manual_seed(seed)
         self.dtype, self.heads, self.kv_heads, self.hd, self.window, self.prefix, self.device = dtype, heads, kv_heads, hd, window, prefix, device
         self.q_lens, self.own_lens = q_lens, own_lens
+        self.page = size = page
         rows = sum(q_lens)
-        counts = [-(-prefix // PAGE)] + [-(-n // PAGE) for n in own_lens]
+        counts = [-(-prefix // size)] + [-(-n // size) for n in own_lens]
         pages = sum(counts) + pool_extra
         perm = torch.randperm(pages, generator=g).tolist()
-        self.k_pool = torch.full((pages, PAGE, kv_heads, hd), float("nan"), dtype=dtype, device=device)
+        self.k_pool = torch.full((pages, size, kv_heads, hd), float("nan"), dtype=dtype, device=device)
         self.v_pool = self.k_pool.clone()
         width = max(counts[1:]) + wider
         at, tables = 0, []
@@ -64,7 +65,7 @@ class Batch:
             at += c
         for table, n in zip(tables, [prefix] + own_lens):
             for lp, page in enumerate(table):
-                here = min(PAGE, n - lp * PAGE)
+                here = min(size, n - lp * size)
                 self.k_pool[page, :here] = torch.randn((here, kv_heads, hd), generator=g).to(dtype).to(device)
                 self.v_pool[page, :here] = torch.randn((here, kv_heads, hd), generator=g).to(dtype).to(device)
         self.prefix_table = torch.tensor(tables[0], dtype=torch.int32, device=device)
@@ -82,7 +83,7 @@ class Batch:
     def run(self, ops, out=None):
         out = self.out if out is None else out
         ops.attention_shared(self.q, self.wide.stride(0), out, self.k_pool, self.v_pool, self.prefix_table, self.prefix, self.block_table,
-                             PAGE, self.row_seq, self.row_pos, self.heads, self.kv_heads, self.hd, self.window, self.scale, self.geometry)
+                             self.page, self.row_seq, self.row_pos, self.heads, self.kv_heads, self.hd, self.window, self.scale, self.geometry)
         return out
 
     def reference(self):
@@ -102,7 +103,7 @@ class Batch:
             seq, pos = int(self.row_seq[r]), int(self.row_pos[r])
             if seq < 0:
                 continue
-            room = self.prefix + self.block_table.shape[1] * PAGE
+            room = self.prefix + self.block_table.shape[1] * self.page
             lo = max(0, pos - self.window + 1) if self.window > 0 else 0
             j = torch.arange(lo, min(pos, room - 1) + 1, device=device)
             if j.numel() == 0:
@@ -110,10 +111,10 @@ class Batch:
             own = j - self.prefix
             table_p = self.prefix_table.long() if self.prefix_table.numel() else torch.zeros(1, dtype=torch.long, device=device)
             table_o = self.block_table[seq].long() if self.block_table.shape[1] else torch.zeros(1, dtype=torch.long, device=device)
-            page = torch.where(own < 0, table_p[(j // PAGE).clamp(max=table_p.numel() - 1)], table_o[(own // PAGE).clamp(0, table_o.numel() - 1)])
-            place = torch.where(own < 0, j, own) % PAGE
+            page = torch.where(own < 0, table_p[(j // self.page).clamp(max=table_p.numel() - 1)], table_o[(own // self.page).clamp(0, table_o.numel() - 1)])
+            place = torch.where(own < 0, j, own) % self.page
             named = (page >= 0) & (page < self.k_pool.shape[0])
-            flat = page.clamp(0, self.k_pool.shape[0] - 1) * PAGE + place
+            flat = page.clamp(0, self.k_pool.shape[0] - 1) * self.page + place
             k = torch.where(named[:, None, None], kf[flat], 0.0)
             v = torch.where(named[:, None, None], vf[flat], 0.0)
             for h in range(self.kv_heads):

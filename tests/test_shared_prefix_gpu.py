@@ -292,10 +292,56 @@ def test_long_prefix_at_the_7b_shape():
     b.check(b.run(ops), "prompts")
 
 
-@pytest.mark.parametrize("heads,kv_heads", [(64, 1), (128, 1), (129, 1), (100, 2)])
-def test_many_heads_on_one_kv_head(heads, kv_heads):
-    b = sp.Batch(BF, [1, 2, 1], [5, 70, 1], 150, heads, kv_heads, 64, seed=heads)
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("heads,kv_heads", [(17, 1), (40, 1), (64, 1), (128, 1), (129, 1), (100, 2)])
+def test_many_heads_on_one_kv_head(dtype, heads, kv_heads):
+    b = sp.Batch(dtype, [1, 2, 1], [5, 70, 1], 150, heads, kv_heads, 64, seed=heads)
     b.check(b.run(ops), "%d heads on %d" % (heads, kv_heads))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("page", [1, 16, 48, 96])
+def test_pages_of_other_sizes(dtype, page):
+    b = sp.Batch(dtype, [1, 3, 1], [1, 70, 200], 130, 14, 2, 64, seed=page, page=page)
+    b.check(b.run(ops), "pages of %d" % page)
+    b = sp.Batch(dtype, [1, 30, 1], [1, 70, 20], 90, 4, 2, 16, window=50, seed=page, page=page)
+    b.check(b.run(ops), "pages of %d, a window" % page)
+
+
+@pytest.mark.parametrize("window", [0, 300])
+def test_more_jobs_than_the_device_takes_at_once(window):
+    """A CTA takes several shares one after another: of unequal lengths, some without keys, some without rows."""
+    lens = [(37 * i * i) % 700 + 1 for i in range(100)]
+    b = sp.Batch(BF, [1] * 100, lens, 2500, 28, 4, 128, window=window, seed=50)
+    b.row_seq[7::13] = -1
+    b.row_pos[3::17] = 100                 # inside the prefix: nothing of their own
+    b.check(b.run(ops), "a hundred sequences")
+    first = b.run(ops).clone()
+    for _ in range(10):
+        b.out.fill_(7.25)
+        assert torch.equal(b.run(ops), first)
+
+
+def test_hundreds_of_sequences():
+    b = sp.Batch(BF, [1] * 333, [i % 90 + 1 for i in range(333)], 400, 6, 3, 16, seed=51)
+    b.check(b.run(ops), "hundreds of sequences")
+    b = sp.Batch(BF, [1 + i % 3 for i in range(250)], [3 + i % 70 for i in range(250)], 65, 8, 8, 32, seed=52)
+    b.check(b.run(ops), "hundreds of short ones")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(28, 4, 128), (14, 2, 64), (2, 2, 20)])
+def test_a_prefix_that_is_still_being_filled(dtype, heads, kv_heads, hd):
+    """Rows inside the prefix, behind which the prefix' pages hold no numbers yet."""
+    for q_lens in ([1, 1, 1], [5, 40, 1]):
+        b = sp.Batch(dtype, q_lens, [q + 3 for q in q_lens], 300, heads, kv_heads, hd, seed=53)
+        far = 205
+        b.row_pos.copy_(torch.arange(len(b.row_pos), device=DEV) * 4 % far)
+        b.row_pos[0] = far
+        flat = torch.arange(far + 1, 300, device=DEV)
+        for pool in (b.k_pool, b.v_pool):
+            pool[b.prefix_table.long()[flat // PAGE], flat % PAGE] = float("nan")
+        b.check(b.run(ops), "half a prefix")
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
@@ -506,7 +552,7 @@ def test_a_document_and_questions_to_it(dtype):
         q = ops.rope_axes_kv_write(qkv, seq, place - prefix, pos, denom, sections, nq, nkv, hd, kp, vp, own_table, PAGE)
         b = sp.Batch.__new__(sp.Batch)
         b.dtype, b.heads, b.kv_heads, b.hd, b.window, b.prefix, b.device = dtype, nq, nkv, hd, 0, prefix, DEV
-        b.k_pool, b.v_pool, b.prefix_table, b.block_table, b.q, b.wide = kp, vp, prefix_table, own_table, q, q
+        b.page, b.k_pool, b.v_pool, b.prefix_table, b.block_table, b.q, b.wide = PAGE, kp, vp, prefix_table, own_table, q, q
         b.row_seq, b.row_pos, b.scale = seq, place, hd ** -0.5
         b.geometry = sp.Geometry([sum(counts[:s]) for s in range(n)], counts, prefix + max(b0 + c for b0, c in zip(begin, counts)), DEV)
         b.out = torch.full((len(seq), nq * hd), 7.25, dtype=dtype, device=DEV)
