@@ -322,6 +322,26 @@ def test_more_jobs_than_the_device_takes_at_once(window):
         assert torch.equal(b.run(ops), first)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 2, 16), (28, 4, 128), (14, 2, 64), (8, 8, 80), (70, 70, 32), (12, 4, 96)])
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 7])
+def test_few_sequences(dtype, heads, kv_heads, hd, n):
+    """One token each, and two for some; rows without a sequence, rows that
+    see nothing, windows, the same bits every time."""
+    b = sp.Batch(dtype, [1] * n, [33 * i + 1 for i in range(n)], 500, heads, kv_heads, hd, seed=60 + n)
+    b.check(b.run(ops), "%d sequences" % n)
+    first = b.run(ops).clone()
+    for _ in range(5):
+        b.out.fill_(7.25)
+        assert torch.equal(b.run(ops), first)
+    b = sp.Batch(dtype, [1 + i % 2 for i in range(n)], [70 * i + 2 for i in range(n)], 129, heads, kv_heads, hd, window=150, seed=70 + n)
+    b.check(b.run(ops), "%d sequences, a window" % n)
+    b.row_seq[0] = -1
+    b.row_pos[-1] = -1
+    b.out.fill_(7.25)
+    b.check(b.run(ops), "%d sequences, rows left out" % n)
+
+
 def test_hundreds_of_sequences():
     b = sp.Batch(BF, [1] * 333, [i % 90 + 1 for i in range(333)], 400, 6, 3, 16, seed=51)
     b.check(b.run(ops), "hundreds of sequences")

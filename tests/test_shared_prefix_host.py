@@ -57,7 +57,7 @@ def shared(rows=2, n_seqs=2, page=64, prefix=70, nq=4, nkv=2, hd=64, window=0, s
     fam = family("attention_shared")
     fn = fam.declare("attention_shared", [P, L, P, P, P, I, I, P, I, P, I, I, P, P, P, P, I, I, I, I, I, I, I, ctypes.c_float, P, L, P, I, P, P])
     launches = I(7)
-    rc = fn(aligned, nq * hd, aligned, aligned, aligned, pool_pages, page, None, prefix, None, n_seqs, width, None, None, None, None, rows, 1, 100, nq, nkv, hd,
+    rc = fn(aligned, nq * hd, aligned, aligned, aligned, pool_pages, page, None, prefix, None, n_seqs, width, None, None, None, None, rows, 1, prefix + 30, nq, nkv, hd,
             window, scale, None, floats, 16, dtype, ctypes.byref(launches), None)
     assert launches.value == 0
     return rc
@@ -65,7 +65,7 @@ def shared(rows=2, n_seqs=2, page=64, prefix=70, nq=4, nkv=2, hd=64, window=0, s
 
 @pytest.mark.parametrize("wrong", [dict(dtype=2), dict(nq=3), dict(nkv=0), dict(hd=0), dict(hd=257), dict(page=0), dict(prefix=-1), dict(window=-1), dict(scale=0.0),
                                    dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(pool_pages=0), dict(width=-1),
-                                   dict(floats=10), dict(floats=10, dtype=0), dict(floats=10, hd=20)])
+                                   dict(floats=10, prefix=20000), dict(floats=10, prefix=20000, dtype=0), dict(floats=10, hd=20)])
 def test_sizes_that_attention_refuses(wrong):
     assert shared(**wrong) == 1
     assert shared(rows=0) == 0 and shared(n_seqs=0) == 0
