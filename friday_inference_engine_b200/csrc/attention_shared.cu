@@ -586,9 +586,15 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 //               scores.  The reference maximum only moves when the true one has grown by more than 8 (in log2 units; weights stay
 //               below 2^8); O is rescaled then.
 //
-// A CTA takes 97 KB of shared memory and half the tensor memory, so two share an SM and one's softmax runs beside the other's
+// A CTA takes 101 KB of shared memory and half the tensor memory, so two share an SM and one's softmax runs beside the other's
 // products: 16 prompts of 2,188 rows in all behind 8,000 keys, 28 heads on 4 of 128, took 250 us this way and 288 with two tiles and
-// blocks of 128 keys in one CTA per SM; 64 one-token rows behind 16,001 keys 52 and 71.  P is rounded to bf16 for the second product
+// blocks of 128 keys in one CTA per SM; 64 one-token rows behind 16,001 keys 52 and 71.  Now 239 us, 0.99 PFLOP/s, the tensor cores
+// active in 0.53 of the cycles and the exponential unit in 0.52: what is left is the chain of a block through one warp's softmax.  (Two
+// groups of warps that take blocks in turn and hand the reference maximum over took 392 us, 96 registers a thread; tiles of few rows on
+// mma.sync, a block of keys per warp, 1.13 us a block of one CTA where this takes 0.68.)
+//
+// Where jobs are more than CTAs, the CTAs stay and take one job of every round, longest first: 64 one-token rows behind 16,001 keys and
+// 1 to 1,000 of their own 38.4 us, 48.5 with a CTA per job.  P is rounded to bf16 for the second product
 // (its sum is not); scores, sums and results are 32-bit.  Values of positions that no row of the CTA sees may be anything: their rows
 // are zeroed in shared memory before the product.  (A position that one row sees and another does not must hold finite values: zero
 // times infinity.)  Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their
@@ -946,7 +952,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             const size_t at = item * p.parts + part;
             if (!p.whole && live) *(float2*)(p.stat + 2 * at) = make_float2(seen ? m_run : -INFINITY, l_run);
             // A part's row leaves through shared memory (every product has read what lay there) as one bulk copy: 16-byte stores of 32
-            // lanes to 32 rows took 3.5 us a CTA, this BULK_TAIL.
+            // lanes to 32 rows took 3.5 us a CTA, this 2.6.
             const int pitch = p.hd * 4 + 16;                   // (eight lanes' pieces fall into different banks)
             uint8_t* const line = smem + r * pitch;
 #pragma unroll 1
