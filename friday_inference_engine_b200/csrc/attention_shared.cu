@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "divide.cuh"
 #include "tc_common.cuh"
 
 FR_EXPORT const char* attention_shared_last_error() { return fr_error_text; }
@@ -51,6 +52,9 @@ struct SharedArgs {
     int whole;                // 1: a CTA walks prefix and own keys of one sequence's rows; 0: CTAs of one or the other, parts joined
     int jobs, prefix_jobs, prefix_splits, own_splits;           // prefix_splits 0: parts are not of one range or the other
     int covered;              // rows of a sequence that the grid's own tiles reach
+    int tiles, own_tiles, tile_tokens;                // row tiles of the prefix' jobs and of a sequence; token rows of a tile
+    // (a CTA's begin is a chain of latencies, of which a dozen divisions by numbers that only the host knows were 0.8 us)
+    FrDivide by_tiles, by_kv, by_seqs, by_inner, by_group, by_heads, by_pieces, by_prefix_splits, by_own_splits;
 };
 
 // the pool's row of position j of sequence `seq`; -1: no page is named
@@ -142,8 +146,8 @@ __global__ void __launch_bounds__(VEC == 4 ? 128 : 256) merge_kernel(const Share
     fr_pdl_launch();
     const int tid = threadIdx.x, lane = tid & 31;
     const long long item = blockIdx.x;
-    const int row = (int)(item / p.nq);
-    const int pieces = p.hd / VEC, at_once = THREADS / pieces, piece = tid % pieces, sub = tid / pieces;
+    const int row = p.by_heads((int)blockIdx.x);
+    const int pieces = p.hd / VEC, at_once = p.by_pieces(THREADS), sub = p.by_pieces(tid), piece = tid - sub * pieces;
     const bool busy = sub < at_once;
     const float* from = p.part + (size_t)item * p.parts * p.hd + piece * VEC;
     float v[AHEAD][VEC];
@@ -264,31 +268,40 @@ __device__ __forceinline__ void order_by_length(const SharedArgs& p, int* s_orde
 // shared memory, (INT_MAX, -1) behind a barrier; s_order: the sequences in the order in which they are taken (null: their own).  For all
 // threads of the block.  early: a share of the prefix without a window does not wait for the rows' positions; its range then ends with
 // the prefix, wherever the last of its rows is.
-__device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int keys, int threads, int* s_pos, const int* s_order, bool early) {
+template <int keys, int threads>
+__device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int* s_pos, const int* s_order, bool early) {
     Job job;
     const bool prefix_job = !p.whole && index < p.prefix_jobs;
-    int share, shares;
+    int share, tile;
     if (prefix_job) {
-        const int per = p.prefix_jobs / (p.nkv * p.prefix_splits);
+        const int q = p.by_tiles(index);
+        tile = index - q * p.tiles;
+        share = p.by_kv(q);
+        job.kvh = q - share * p.nkv;
         job.seq = 0;
-        job.row0 = index % per * T;
-        job.kvh = index / per % p.nkv;
-        share = index / (per * p.nkv);
-        shares = p.prefix_splits;
+        job.row0 = tile * T;
         job.part = share;
         job.n_tok = min(T, p.rows - job.row0);
     } else {
-        const int x = index - p.prefix_jobs;
-        shares = p.whole ? 1 : p.own_splits;
-        const int per = (p.jobs - p.prefix_jobs) / (p.n_seqs * p.nkv * shares);
         // (whole: the sequences' tiles of one rank together; else the shares and kv heads of a sequence)
-        const int inner = p.whole ? p.n_seqs : p.nkv * shares;
-        const int s = p.whole ? x % inner : x / inner % p.n_seqs, rest = p.whole ? x / inner % p.nkv : x % inner;
+        const int x = index - p.prefix_jobs;
+        int s;
+        if (p.whole) {
+            const int q = p.by_seqs(x);
+            s = x - q * p.n_seqs;
+            tile = p.by_kv(q);
+            job.kvh = q - tile * p.nkv;
+            share = 0;
+        } else {
+            const int q = p.by_inner(x), rest = x - q * (int)p.by_inner.by;
+            tile = p.by_seqs(q);
+            s = q - tile * p.n_seqs;
+            share = p.by_kv(rest);
+            job.kvh = rest - share * p.nkv;
+        }
         job.seq = s_order != nullptr ? s_order[s] : s;
-        job.kvh = rest % p.nkv;
-        share = rest / p.nkv;
         job.part = p.prefix_splits + share;
-        const int t0 = (per - 1 - x / (p.n_seqs * p.nkv * shares)) * T;
+        const int t0 = (p.own_tiles - 1 - tile) * T;
         const int begin = p.seq_start[job.seq], count = begin < 0 || begin > p.rows ? 0 : min(p.seq_qlen[job.seq], p.rows - begin);
         job.row0 = begin + t0;
         job.n_tok = max(0, min(T, count - t0));
@@ -314,12 +327,14 @@ __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int
         if (p.whole || prefix_job) job.seg0.hi = min(most, p.prefix - 1);
         if (!prefix_job) job.seg1.hi = most - p.prefix;
     }
+    // equal shares of the blocks, the first ones a block longer where they do not come out even
+    const FrDivide& shares = prefix_job ? p.by_prefix_splits : p.by_own_splits;
     auto take_share = [&](Range& g) {
         if (g.hi < g.lo) return;
         const int first = g.lo / keys, n = g.hi / keys - first + 1;
-        const int from = (int)((long long)n * share / shares), to = (int)((long long)n * (share + 1) / shares);
-        g.first = first + from;
-        g.n = to - from;
+        const int each = shares(n), more = n - each * (int)shares.by;
+        g.first = first + share * each + min(share, more);
+        g.n = each + (share < more ? 1 : 0);
     };
     take_share(job.seg0);
     take_share(job.seg1);
@@ -358,8 +373,8 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
     __syncthreads();
     fr_pdl_wait();
     fr_pdl_launch();
-    const int G = p.nq / p.nkv, T = ROWS / G;
-    const Job job = job_of(p, (int)blockIdx.x, T, KEYS, THREADS, s_pos, nullptr, false);
+    const int G = (int)p.by_group.by, T = p.tile_tokens;
+    const Job job = job_of<KEYS, THREADS>(p, (int)blockIdx.x, T, s_pos, nullptr, false);
     const int n_rows = job.n_tok * G, n_blocks = job.seg0.n + job.seg1.n;
     auto range_of = [&](int i, int& j0, bool& own) {
         own = i >= job.seg0.n;
@@ -407,7 +422,8 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
     for (int idx = tid; idx < ROWS * (HD / 4); idx += THREADS) {
         const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < n_rows && c < p.hd) v = *(const float4*)((const float*)p.q + (size_t)(job.row0 + r / G) * p.q_stride + (size_t)(job.kvh * G + r % G) * p.hd + c);
+        const int t = p.by_group(r);
+        if (r < n_rows && c < p.hd) v = *(const float4*)((const float*)p.q + (size_t)(job.row0 + t) * p.q_stride + (size_t)(job.kvh * G + r - t * G) * p.hd + c);
         v.x *= p.scale_log2; v.y *= p.scale_log2; v.z *= p.scale_log2; v.w *= p.scale_log2;
         *(float4*)(sq + r * LQ + c) = v;
     }
@@ -421,9 +437,9 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
         live[i] = r < n_rows;
         pos[i] = -1;
         if (live[i]) {
-            const int of = p.row_seq[job.row0 + r / G];
+            const int row = job.row0 + p.by_group(r), of = p.row_seq[row];
             live[i] = of >= 0 && of < p.n_seqs;
-            if (live[i]) pos[i] = position_of(p, job.row0 + r / G);
+            if (live[i]) pos[i] = position_of(p, row);
         }
         first[i] = fr_first_key(pos[i], p.window, 0);
         m[i] = -INFINITY;
@@ -539,8 +555,8 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
 #pragma unroll
     for (int a = 0; a < RPT; ++a) {
         if (!live[a]) continue;
-        const int r = r0 + 16 * a;
-        const size_t item = (size_t)(job.row0 + r / G) * p.nq + (size_t)job.kvh * G + r % G, at = item * p.parts + job.part;
+        const int r = r0 + 16 * a, t = p.by_group(r);
+        const size_t item = (size_t)(job.row0 + t) * p.nq + (size_t)job.kvh * G + r - t * G, at = item * p.parts + job.part;
         const float inv = l[a] > 0.f ? 1.f / l[a] : l[a];              // (nothing seen: 0; a NaN stays one)
         float* to = p.whole ? (float*)p.out + item * p.hd : p.part + at * p.hd;
         if (!p.whole && tx == 0) *(float2*)(p.stat + 2 * at) = make_float2(m[a], l[a]);
@@ -736,7 +752,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     fr_pdl_wait();
     if (threadIdx.x == 0) fr_pdl_launch();
 
-    const int G = p.nq / p.nkv, T = ROWS / G;         // token rows of a tile
+    const int G = (int)p.by_group.by, T = p.tile_tokens;
     const int slices = (p.hd + 63) / 64;
     int* s_order = nullptr;
     if (!p.whole && p.n_seqs <= THREADS && p.jobs > (int)gridDim.x) {
@@ -751,7 +767,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if ((long long)round * gridDim.x >= p.jobs) break;
     if (index >= p.jobs) continue;
     int* const s_range = s_pos + 1 + 2 * (round & 1);
-    const Job job = job_of(p, (int)index, T, KEYS, THREADS, s_range, s_order, true);
+    const Job job = job_of<KEYS, THREADS>(p, (int)index, T, s_range, s_order, true);
     const Range seg0 = job.seg0, seg1 = job.seg1;
     const int kvh = job.kvh, seq = job.seq, row0 = job.row0, n_tok = job.n_tok, part = job.part;
     const int n_blocks = seg0.n + seg1.n, before = blocks_before;
@@ -833,7 +849,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
     } else {
         const int quarter = warp & 3;                          // the tensor-memory lanes that this warp may touch: 32 * quarter ..
-        const int r = quarter * 32 + lane, t = r / G, g = r - t * G;
+        const int r = quarter * 32 + lane, t = p.by_group(r), g = r - t * G;
         const int row = row0 + t;
         int pos = -1;
         bool live = r < T * G && t < n_tok;
@@ -1239,7 +1255,15 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
         p.whole = plan.whole; p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits;
         p.jobs = (int)plan.ctas;
         p.prefix_jobs = plan.whole ? 0 : plan.tiles * nkv * plan.prefix_splits;
-        p.covered = plan.own_tiles * (kind.rows / (nq / nkv));
+        p.tiles = plan.tiles; p.own_tiles = plan.own_tiles; p.tile_tokens = kind.rows / (nq / nkv);
+        p.covered = plan.own_tiles * p.tile_tokens;
+        p.by_tiles = FrDivide(p.tiles, p.jobs);
+        p.by_kv = FrDivide(nkv, p.jobs);
+        p.by_seqs = FrDivide(n_seqs, p.jobs);
+        p.by_inner = FrDivide((long long)nkv * (plan.whole ? 1 : plan.own_splits), p.jobs);
+        p.by_group = FrDivide(nq / nkv, kind.rows);
+        p.by_prefix_splits = FrDivide(plan.whole ? 1 : plan.prefix_splits, 0x7fffffff / kind.keys + 1);
+        p.by_own_splits = FrDivide(plan.whole ? 1 : plan.own_splits, 0x7fffffff / kind.keys + 1);
         const int rc = dtype == FR_BF16 ? tcore::launch(p, plan.ctas, stream)
                        : hd <= 32       ? f32::launch_rows<32>(p, kind.rows, plan.ctas, stream)
                        : hd <= 64       ? f32::launch_rows<64>(p, kind.rows, plan.ctas, stream)
@@ -1252,6 +1276,8 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     *launches = 1;
     if (plan.parts > 1) {
         const dim3 grid((unsigned)((long long)rows * nq));
+        p.by_heads = FrDivide(nq, (long long)rows * nq);
+        p.by_pieces = FrDivide(hd % 4 == 0 ? hd / 4 : hd, 256);
         if (dtype == FR_F32 && hd % 4 == 0) FR_CUDA(fr_launch(merge_kernel<float, 4>, grid, dim3(128), 0, stream, p));
         else if (dtype == FR_F32) FR_CUDA(fr_launch(merge_kernel<float, 1>, grid, dim3(256), 0, stream, p));
         else if (hd % 4 == 0) FR_CUDA(fr_launch(merge_kernel<bf16, 4>, grid, dim3(128), 0, stream, p));

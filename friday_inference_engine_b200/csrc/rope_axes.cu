@@ -14,6 +14,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "divide.cuh"
 #include "tc_common.cuh"
 
 FR_EXPORT const char* rope_axes_last_error() { return fr_error_text; }
@@ -125,17 +126,10 @@ __global__ void __launch_bounds__(256) rope_axes_single_kernel(const RopeArgs p)
 // 256 rows x 32 heads of 80 3.1 us.
 constexpr int AHEAD = 4, THREADS = 256, MOST_ROWS = 32;
 
-// n / by as the upper half of n * ceil(2^32 / by): exact while n * by < 2^32
-struct Divide {
-    unsigned by, magic;
-    Divide(unsigned n = 1) : by(n), magic(n > 1 ? (unsigned)(((1ull << 32) + n - 1) / n) : 0) {}
-    __device__ __forceinline__ int operator()(int n) const { return by == 1 ? n : (int)__umulhi((unsigned)n, magic); }
-};
-
 struct Units {
     int rows, turn, stay;                             // rows of a block; where a row's units that turn end, and those that stay
-    Divide all, half;                                 // units of a row; pairs of a head
-    Divide turn_pieces, stay_pieces, value_pieces;    // units of a head
+    FrDivide all, half;                               // units of a row; pairs of a head
+    FrDivide turn_pieces, stay_pieces, value_pieces;    // units of a head
 };
 
 template <typename T, int VEC>
@@ -160,19 +154,19 @@ __global__ void __launch_bounds__(THREADS) rope_axes_kernel(const RopeArgs p, co
     };
     auto unit_of = [&](int idx) {
         Unit u;
-        u.local = un.all(idx);
+        u.local = un.all.quick(idx);
         int k = idx - u.local * (int)un.all.by;
         u.turns = k < un.turn;
         if (u.turns) {
-            u.head = un.turn_pieces(k);
+            u.head = un.turn_pieces.quick(k);
             u.off = (k - u.head * (int)un.turn_pieces.by) * VEC;
         } else if (k < un.stay) {
             k -= un.turn;
-            u.head = un.stay_pieces(k);
+            u.head = un.stay_pieces.quick(k);
             u.off = 2 * p.half + (k - u.head * (int)un.stay_pieces.by) * VEC;
         } else {
             k -= un.stay;
-            u.head = un.value_pieces(k);
+            u.head = un.value_pieces.quick(k);
             u.off = (k - u.head * (int)un.value_pieces.by) * VEC;
             u.head += turning;
         }
@@ -192,7 +186,7 @@ __global__ void __launch_bounds__(THREADS) rope_axes_kernel(const RopeArgs p, co
     };
     fetch(threadIdx.x);
     for (int idx = threadIdx.x; idx < rows * p.half; idx += THREADS) {
-        const int r = un.half(idx), i = idx - r * p.half, at = i / PAIRS, j = i - at * PAIRS;
+        const int r = un.half.quick(idx), i = idx - r * p.half, at = i / PAIRS, j = i - at * PAIRS;
         float s, c;
         sin_cos_at(turn_step(p.denom[i]), p.positions[(size_t)(row0 + r) * p.axes + axis_of(p, i)], s, c);
         table[r * p.half + (PAIRS == 1 ? at : 2 * ((j >> 1) * (int)un.turn_pieces.by + at) + (j & 1))] = make_float2(c, s);
@@ -313,7 +307,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
         for (int i = 0; i < RING_ANGLES; ++i) {
             const int idx = tid + i * RING_THREADS;
             if (idx < rows * p.half) {
-                const int r = un.half(idx);
+                const int r = un.half.quick(idx);
                 pos[i] = p.positions[(size_t)(row0 + r) * p.axes + s_axis[idx - r * p.half]];
             }
         }
@@ -331,7 +325,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
         for (int i = 0; i < RING_ANGLES; ++i) {
             const int idx = tid + i * RING_THREADS;
             if (idx < rows * p.half) {
-                const int r = un.half(idx), pair = idx - r * p.half, at = pair / PAIRS, j = pair - at * PAIRS;
+                const int r = un.half.quick(idx), pair = idx - r * p.half, at = pair / PAIRS, j = pair - at * PAIRS;
                 float s, c;
                 sin_cos_at(s_step[pair], pos[i], s, c);
                 table[r * p.half + (PAIRS == 1 ? at : 2 * ((j >> 1) * (int)un.turn_pieces.by + at) + (j & 1))] = make_float2(c, s);
@@ -353,7 +347,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
         uint8_t* stage = ring + b * stage_bytes;
         const float2* table = tables + (k & 1) * un.rows * p.half;
         for (int idx = tid; idx < rows * un.turn; idx += RING_THREADS) {
-            const int r = un.all(idx), u = idx - r * un.turn, head = un.turn_pieces(u), unit = u - head * (int)un.turn_pieces.by;
+            const int r = un.all.quick(idx), u = idx - r * un.turn, head = un.turn_pieces.quick(u), unit = u - head * (int)un.turn_pieces.by;
             T* at = (T*)(stage + r * row_bytes) + head * p.hd + unit * VEC;
             P a = *(const P*)at, b2;
             if (!NEIGHBOURS) b2 = *(const P*)(at + p.half);
@@ -425,11 +419,12 @@ cudaError_t launch_pieces(const RopeArgs& p, cudaStream_t stream) {
     un.turn = heads * turn;
     un.stay = un.turn + heads * stay;
     const int all = un.stay + p.nkv * (p.hd / VEC);
-    un.all = Divide(all);
-    un.half = Divide(p.half);
-    un.turn_pieces = Divide(turn);
-    un.stay_pieces = Divide(stay > 0 ? stay : 1);
-    un.value_pieces = Divide(p.hd / VEC);
+    // (several rows only where all of their units are a block's)
+    un.all = FrDivide(all, all > AHEAD * THREADS ? all : AHEAD * THREADS);
+    un.half = FrDivide(p.half, MOST_ROWS * MOST_HALF);
+    un.turn_pieces = FrDivide(turn, all);
+    un.stay_pieces = FrDivide(stay > 0 ? stay : 1, all);
+    un.value_pieces = FrDivide(p.hd / VEC, all);
     // as many rows as give every thread its four units, while there are more blocks than the device takes at once
     const int sms = fr_sm_count() > 0 ? fr_sm_count() : 148;
     const int fit = AHEAD * THREADS / all, spread = p.rows / (4 * sms);
@@ -476,9 +471,9 @@ cudaError_t launch_ring(const RopeArgs& p, cudaStream_t stream) {
     if (un.rows > RING_ROWS) un.rows = RING_ROWS;
     if (un.rows > RING_ANGLES * RING_THREADS / p.half) un.rows = RING_ANGLES * RING_THREADS / p.half;
     un.turn = un.stay = (p.nq + p.nkv) * turn;
-    un.all = Divide(un.turn);
-    un.half = Divide(p.half);
-    un.turn_pieces = Divide(turn);
+    un.all = FrDivide(un.turn, (long long)un.rows * un.turn);
+    un.half = FrDivide(p.half, (long long)un.rows * p.half);
+    un.turn_pieces = FrDivide(turn, un.turn);
     const int stage = un.rows * row_bytes, tables = 2 * un.rows * p.half * (int)sizeof(float2);
     return 4 * stage <= RING_BYTES ? launch_ring_of<T, VEC, NEIGHBOURS, 4>(p, un, 4 * stage + tables, stream)
                                    : launch_ring_of<T, VEC, NEIGHBOURS, 3>(p, un, 3 * stage + tables, stream);
@@ -487,7 +482,7 @@ cudaError_t launch_ring(const RopeArgs& p, cudaStream_t stream) {
 // The widest piece (16, 8 or 4 bytes) that every head's parts, rows and starts are made of; 0: none.
 template <typename T>
 int piece_bytes(const RopeArgs& p) {
-    if ((long long)(p.nq + 2 * p.nkv) * p.hd >= 65536) return 0;       // (beyond Divide: units of a row squared stay below 2^32)
+    if ((long long)(p.nq + 2 * p.nkv) * p.hd >= 65536) return 0;       // (FrDivide::quick: units of a row squared stay below 2^32)
     for (int bytes = 16; bytes >= 4; bytes /= 2) {
         const int vec = bytes / (int)sizeof(T);
         if (p.neighbours && vec < 2) break;
