@@ -240,6 +240,7 @@ struct Job {
     int kvh, seq, row0, n_tok, part;      // n_tok token rows from row0 on
     Range seg0, seg1;                     // of the prefix; of own keys, numbered from the prefix' end
     bool early;
+    int first_page;                       // of own keys, looked up while the rows' positions are on the way (-2: not looked up)
 };
 
 // The sequences by their last position, greatest first (ties: the lower number first): own jobs are taken longest first.
@@ -271,6 +272,7 @@ __device__ __forceinline__ void order_by_length(const SharedArgs& p, int* s_orde
 template <int keys, int threads>
 __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int* s_pos, const int* s_order, bool early) {
     Job job;
+    job.first_page = -2;
     const bool prefix_job = !p.whole && index < p.prefix_jobs;
     int share, tile;
     if (prefix_job) {
@@ -301,6 +303,8 @@ __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int
         }
         job.seq = s_order != nullptr ? s_order[s] : s;
         job.part = p.prefix_splits + share;
+        // (without a window the first share begins with the first page)
+        if (!p.whole && share == 0 && p.window == 0 && p.table_width > 0) job.first_page = p.block_table[(size_t)job.seq * p.table_width];
         const int t0 = (p.own_tiles - 1 - tile) * T;
         const int begin = p.seq_start[job.seq], count = begin < 0 || begin > p.rows ? 0 : min(p.seq_qlen[job.seq], p.rows - begin);
         job.row0 = begin + t0;
@@ -311,16 +315,22 @@ __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int
     if (job.early) {
         job.seg0.hi = p.prefix - 1;
     } else {
-        for (int t = threadIdx.x; t < job.n_tok; t += threads) {
-            const int of = p.row_seq[job.row0 + t];
-            if (of >= 0 && of < p.n_seqs) {
-                const int pos = position_of(p, job.row0 + t);
-                atomicMin(&s_pos[0], pos);
-                atomicMax(&s_pos[1], pos);
+        int least = 0x7fffffff, most = -1;
+        if (job.n_tok == 1) {                                      // (a one-token step: every thread looks for itself)
+            const int of = p.row_seq[job.row0], pos = position_of(p, job.row0);
+            if (of >= 0 && of < p.n_seqs) least = most = pos;
+        } else {
+            for (int t = threadIdx.x; t < job.n_tok; t += threads) {
+                const int of = p.row_seq[job.row0 + t], pos = position_of(p, job.row0 + t);
+                if (of >= 0 && of < p.n_seqs) {
+                    atomicMin(&s_pos[0], pos);
+                    atomicMax(&s_pos[1], pos);
+                }
             }
+            __syncthreads();
+            least = s_pos[0];
+            most = s_pos[1];
         }
-        __syncthreads();
-        const int least = s_pos[0], most = s_pos[1];
         const int lo = most < 0 ? 0 : fr_first_key(least, p.window, 0);
         job.seg0.lo = lo;
         job.seg1.lo = max(0, lo - p.prefix);
@@ -786,7 +796,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 if (!mbar_wait(empty + 8 * b, par ^ 1, p.status, 1)) return false;
                 mbar_expect_tx(full + 8 * b, (uint32_t)(slices * KSLICE));
                 const int* table = i < seg0.n ? p.prefix_table : p.block_table + (size_t)seq * p.table_width;
-                int page = table[first_key_of(i) / PAGE];
+                int page = i == 0 && job.first_page != -2 ? job.first_page : table[first_key_of(i) / PAGE];
                 if (page < 0 || page >= p.pool_pages) page = p.pool_pages;              // beyond the pool: zeros
                 for (int s = 0; s < slices; ++s)
                     load_3d(smem_u32(ring) + (uint32_t)(b * STAGE + s * KSLICE), map, s * 64, kvh, page * PAGE, full + 8 * b);
