@@ -247,13 +247,14 @@ __global__ void __launch_bounds__(THREADS) rope_axes_kernel(const RopeArgs p, co
 // The same units, worked on in shared memory: a block goes through groups of rows, which bulk copies bring into a ring of stages and take
 // from there to the queries' rows and the cache's; what is on the way never waits for what is being turned.  In a group's round its
 // pieces are turned in place, the sines and cosines of the next group are made (from positions that were fetched a round before), and
-// one thread sends the group off and refills the stage of the group before.  Three blocks
+// one warp sends the group off and refills the stage of the group before, a lane per row (one thread for all rows, 16 of them at most:
+// 44,001 rows x 2 heads of 72, bf16, 22.4 us for 14.8; 9,000 rows of 5 heads of 32 into the cache 9.8 for 7.3).  Three blocks
 // per SM with stages of up to 22 KB: 65,536 rows x 32 heads of 80, bf16, 114 us (5.9 TB/s, 0.90 of the measured copy; 133 with two blocks
 // and 20 KB, 219 with the kernel above, whose blocks wait for memory, for positions and for one another in turn); 32,770 rows of 56 heads
 // of 128 into the cache 164 us (352 above).
-constexpr int RING_THREADS = 256, RING_BLOCKS = 3, RING_ROWS = 16;
-constexpr int RING_ANGLES = 2;                                     // sines and cosines that a thread makes per group, at most
-constexpr int STAGE_BYTES = 22 * 1024, RING_BYTES = 66 * 1024;     // of a group, of all stages
+constexpr int RING_THREADS = 256, RING_BLOCKS = 3, RING_ROWS = 64;
+constexpr int RING_ANGLES = 4;                                     // sines and cosines that a thread makes per group, at most
+constexpr int STAGE_BYTES = 22 * 1024, RING_BYTES = 71 * 1024;     // of a group; of all stages and the tables (three blocks per SM)
 // Bytes of rows: below, the kernel above (28 heads on 4 of 128, bf16, us, above / ring: 64 rows 4.08 / 3.94, 200 rows 4.5 / 4.0, 500 rows
 // 7.3 / 5.0; 32 heads of 80: 64 rows 2.9 / 3.9, 200 rows 3.2 / 4.0, 500 rows 4.9 / 4.1).
 constexpr long long RING_FROM = 2 << 20;
@@ -289,12 +290,13 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
     }
     __syncthreads();
     const int groups = (p.rows + un.rows - 1) / un.rows;
-    auto load = [&](int k) {                                   // one thread's: the block's k-th group
+    auto load = [&](int k) {                                   // the first warp's: the block's k-th group
         const long long g = (long long)blockIdx.x + (long long)k * gridDim.x;
         if (g >= groups) return;
         const int row0 = (int)g * un.rows, rows = min(un.rows, p.rows - row0), b = k % STAGES;
-        tc::mbar_expect_tx(full + 8 * b, (uint32_t)(rows * row_bytes));
-        for (int r = 0; r < rows; ++r)
+        if (tid == 0) tc::mbar_expect_tx(full + 8 * b, (uint32_t)(rows * row_bytes));
+        __syncwarp();
+        for (int r = tid; r < rows; r += 32)
             bulk_in(ring0 + (uint32_t)(b * stage_bytes + r * row_bytes), (const T*)p.x + (size_t)(row0 + r) * p.ld, (uint32_t)row_bytes, full + 8 * b);
     };
     // what a group's sines, cosines and places are made from
@@ -306,6 +308,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
 #pragma unroll
         for (int i = 0; i < RING_ANGLES; ++i) {
             const int idx = tid + i * RING_THREADS;
+            if (i > 0 && i * RING_THREADS >= un.rows * p.half) break;
             if (idx < rows * p.half) {
                 const int r = un.half.quick(idx);
                 pos[i] = p.positions[(size_t)(row0 + r) * p.axes + s_axis[idx - r * p.half]];
@@ -324,6 +327,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
 #pragma unroll
         for (int i = 0; i < RING_ANGLES; ++i) {
             const int idx = tid + i * RING_THREADS;
+            if (i > 0 && i * RING_THREADS >= un.rows * p.half) break;
             if (idx < rows * p.half) {
                 const int r = un.half.quick(idx), pair = idx - r * p.half, at = pair / PAIRS, j = pair - at * PAIRS;
                 float s, c;
@@ -333,7 +337,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
         }
         if (tid < rows) s_at[k & 1][tid] = seq < 0 ? -2 : p.nkv > 0 ? cache_row(p, seq, place) : -1;
     };
-    if (tid == 0)
+    if (tid < 32)
         for (int k = 0; k < STAGES - 1; ++k) load(k);
     fetch(0);
     angles(0);
@@ -377,8 +381,8 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
         angles(k + 1);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
-        if (tid == 0) {
-            for (int r = 0; r < rows; ++r) {
+        if (tid < 32) {
+            for (int r = tid; r < rows; r += 32) {
                 const long long at = s_at[k & 1][r];
                 if (at == -2) continue;
                 const uint32_t from = ring0 + (uint32_t)(b * stage_bytes + r * row_bytes);
@@ -391,10 +395,11 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             // the group before has left its stage: the next group to come takes it
             asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            __syncwarp();
             load(k + STAGES - 1);
         }
     }
-    if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (tid < 32) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 int check(const RopeArgs& p, int dtype, const int* sections) {
@@ -453,7 +458,7 @@ cudaError_t launch_ring_of(const RopeArgs& p, const Units& un, int smem, cudaStr
     const unsigned long long bit = 1ull << (device & 63);
     if (!(configured.load() & bit)) {
         e = cudaFuncSetAttribute(rope_axes_ring_kernel<T, VEC, NEIGHBOURS, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 RING_BYTES + 2 * RING_ANGLES * RING_THREADS * (int)sizeof(float2));
+                                 RING_BYTES);
         if (e != cudaSuccess) return e;
         configured.fetch_or(bit);
     }
@@ -469,14 +474,19 @@ cudaError_t launch_ring(const RopeArgs& p, cudaStream_t stream) {
     const int row_bytes = (p.nq + 2 * p.nkv) * p.hd * (int)sizeof(T), turn = p.half / PAIRS;
     un.rows = STAGE_BYTES / row_bytes;
     if (un.rows > RING_ROWS) un.rows = RING_ROWS;
+    // (no more rows than leave a group for every block)
+    const int blocks = RING_BLOCKS * (fr_sm_count() > 0 ? fr_sm_count() : 148), share = (p.rows + blocks - 1) / blocks;
+    if (un.rows > share) un.rows = share;
     if (un.rows > RING_ANGLES * RING_THREADS / p.half) un.rows = RING_ANGLES * RING_THREADS / p.half;
+    // (three stages and the tables have to fit; a row's tables are at most 2 KB)
+    while (un.rows > 1 && un.rows * (3 * row_bytes + 2 * p.half * (int)sizeof(float2)) > RING_BYTES) --un.rows;
     un.turn = un.stay = (p.nq + p.nkv) * turn;
     un.all = FrDivide(un.turn, (long long)un.rows * un.turn);
     un.half = FrDivide(p.half, (long long)un.rows * p.half);
     un.turn_pieces = FrDivide(turn, un.turn);
     const int stage = un.rows * row_bytes, tables = 2 * un.rows * p.half * (int)sizeof(float2);
-    return 4 * stage <= RING_BYTES ? launch_ring_of<T, VEC, NEIGHBOURS, 4>(p, un, 4 * stage + tables, stream)
-                                   : launch_ring_of<T, VEC, NEIGHBOURS, 3>(p, un, 3 * stage + tables, stream);
+    return 4 * stage + tables <= RING_BYTES ? launch_ring_of<T, VEC, NEIGHBOURS, 4>(p, un, 4 * stage + tables, stream)
+                                            : launch_ring_of<T, VEC, NEIGHBOURS, 3>(p, un, 3 * stage + tables, stream);
 }
 
 // The widest piece (16, 8 or 4 bytes) that every head's parts, rows and starts are made of; 0: none.
