@@ -614,13 +614,14 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 //
 // A CTA takes 101 KB of shared memory and half the tensor memory, so two share an SM and one's softmax runs beside the other's
 // products: 16 prompts of 2,188 rows in all behind 8,000 keys, 28 heads on 4 of 128, took 250 us this way and 288 with two tiles and
-// blocks of 128 keys in one CTA per SM; 64 one-token rows behind 16,001 keys 52 and 71.  Now 239 us, 0.99 PFLOP/s, the tensor cores
-// active in 0.53 of the cycles and the exponential unit in 0.52: what is left is the chain of a block through one warp's softmax.  (Two
-// groups of warps that take blocks in turn and hand the reference maximum over took 392 us, 96 registers a thread; tiles of few rows on
+// blocks of 128 keys in one CTA per SM; 64 one-token rows behind 16,001 keys 52 and 71.  Now 238 us, 0.99 PFLOP/s: 784 cycles a
+// block of an SM, of which the first product's instructions take 8 x 48 (at 64 keys each reads twice as much of Q as of K) and the
+// second's 4 x 64.  (A fourth of the exponentials as polynomials changes nothing; scores fetched at once so that one buffer serves, with
+// half of Q in tensor memory, 276 us; two threads per row 290.  Two groups of warps that take blocks in turn and hand the reference maximum over took 392 us, 96 registers a thread; tiles of few rows on
 // mma.sync, a block of keys per warp, 1.13 us a block of one CTA where this takes 0.68.)
 //
 // Where jobs are more than CTAs, the CTAs stay and take one job of every round, longest first: 64 one-token rows behind 16,001 keys and
-// 1 to 1,000 of their own 38.4 us, 48.5 with a CTA per job.  P is rounded to bf16 for the second product
+// 1 to 1,000 of their own 37 us, 48.5 with a CTA per job.  P is rounded to bf16 for the second product
 // (its sum is not); scores, sums and results are 32-bit.  Values of positions that no row of the CTA sees may be anything: their rows
 // are zeroed in shared memory before the product.  (A position that one row sees and another does not must hold finite values: zero
 // times infinity.)  Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their
