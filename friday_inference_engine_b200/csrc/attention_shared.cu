@@ -617,8 +617,9 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 // blocks of 128 keys in one CTA per SM; 64 one-token rows behind 16,001 keys 52 and 71.  Now 238 us, 0.99 PFLOP/s: 784 cycles a
 // block of an SM, of which the first product's instructions take 8 x 48 (at 64 keys each reads twice as much of Q as of K) and the
 // second's 4 x 64.  (A fourth of the exponentials as polynomials changes nothing; scores fetched at once so that one buffer serves, with
-// half of Q in tensor memory, 276 us; two threads per row 290.  Two groups of warps that take blocks in turn and hand the reference maximum over took 392 us, 96 registers a thread; tiles of few rows on
-// mma.sync, a block of keys per warp, 1.13 us a block of one CTA where this takes 0.68.)
+// half of Q in tensor memory, 276 us; two threads per row 290.  Two groups of warps that take blocks in turn and hand the reference
+// maximum over took 392 us, 96 registers a thread; tiles of few rows on mma.sync, a block of keys per warp, 1.13 us a block of one CTA
+// where this takes 0.68.)
 //
 // Where jobs are more than CTAs, the CTAs stay and take one job of every round, longest first: 64 one-token rows behind 16,001 keys and
 // 1 to 1,000 of their own 37 us, 48.5 with a CTA per job.  P is rounded to bf16 for the second product
@@ -1258,6 +1259,7 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
                        pool_pages < 0x7fffffff / tcore::PAGE && status != nullptr;
     const Plan plan = tiles ? plan_tiles(kind, rows, n_seqs, max_q_len, max_kv_len, prefix, nq, nkv, hd, window) : plan_rows(rows, nq, max_kv_len, window);
     if (scratch_floats < floats_of(plan, rows, nq, hd)) FR_REFUSE("attention_shared: %lld floats of working memory are too few", scratch_floats);
+    if (plan.parts > 1 && (scratch == nullptr || ((uintptr_t)scratch & 15) != 0)) FR_REFUSE("attention_shared: working memory begins on a 16-byte boundary");
     p.parts = plan.parts;
     p.part = scratch;
     p.stat = scratch + ((long long)rows * nq * plan.parts * hd + 1) / 2 * 2;           // (pairs of numbers)

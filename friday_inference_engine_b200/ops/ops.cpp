@@ -1735,6 +1735,7 @@ bool rows_collide(const Tensor& a, int64_t na, const Tensor& b, int64_t nb, bool
 void check_rows(const char* what, const Tensor& t, int64_t columns) {
     if (t.ndim != 2 || (t.dtype != DType::F32 && t.dtype != DType::BF16) || t.cols() < columns || (t.rows() > 1 && t.ld < t.cols()))
         throw KernelError(format("%s: rows of float32 or bfloat16 with at least %lld columns are wanted", what, (long long)columns));
+    if (t.rows() > 0 && !t.data) throw KernelError(format("%s: rows without an address", what));
 }
 
 void check_axes(const char* what, const Ops::AxesSpec& s, const int* positions) {

@@ -1,5 +1,6 @@
 """Rotary positions with several axes, their append to the paged cache, attention of a batch with a shared prefix: against their
 definitions in 64-bit, at the sizes, masks and layouts where each can go wrong, and as they are used one after another."""
+import ctypes
 import threading
 
 import pytest
@@ -603,6 +604,23 @@ def test_a_document_and_questions_to_it(dtype):
 
 
 # ------------------------------------------------------------------ refusals
+def test_rows_without_an_address_are_refused():
+    lib, backend = native.lib(), ops.backend()
+    P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+    x, one = torch.zeros((2, 64), device=DEV), torch.zeros(64, dtype=torch.int32, device=DEV)
+    ones, pool = torch.ones(32, device=DEV), torch.zeros((1, PAGE, 1, 64), device=DEV)
+    at = [P(t.data_ptr()) for t in (x, one, ones, pool)]
+    sections, h = (I * 1)(32), P(backend._h.value)
+    rotate, append, shared = (getattr(lib, "friday_ops_" + n) for n in ("rotate_axes", "rope_axes_kv_write", "attention_shared"))
+    for a, b in ((None, at[0]), (at[0], None)):
+        assert rotate(h, a, L(2), L(64), L(64), b, L(2), L(64), L(64), I(0), at[1], at[2], sections, I(1), I(0), I(0), I(1), I(64), None) != 0
+        assert shared(h, a, L(2), L(64), L(64), b, L(2), L(64), I(0), at[3], at[3], I(1), I(PAGE), None, I(0), at[1], I(1), I(1), at[1], at[1], at[1], at[1],
+                      I(2), I(2), I(1), I(1), I(64), I(0), F(0.1), None, L(0), None) != 0
+    assert append(h, None, L(2), L(192), L(192), at[0], L(2), L(64), L(64), I(0), at[1], at[1], at[1], at[2], sections, I(1), I(0), I(0), I(1), I(1),
+                  I(64), at[3], at[3], I(1), I(PAGE), at[1], I(1), I(1), None) != 0
+    backend.check_status()
+
+
 def test_refusals():
     b = sp.Batch(BF, [1, 1], [4, 5], 70, 14, 2, 64, seed=40)
     args = dict(q=b.q, q_stride=b.wide.stride(0), out=b.out, k_pool=b.k_pool, v_pool=b.v_pool, prefix_table=b.prefix_table, prefix_len=70,

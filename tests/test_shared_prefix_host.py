@@ -71,6 +71,17 @@ def test_sizes_that_attention_refuses(wrong):
     assert shared(rows=0) == 0 and shared(n_seqs=0) == 0
 
 
+def test_working_memory_that_is_missing_or_begins_anywhere_is_refused():
+    fam = family("attention_shared")
+    fn = fam.declare("attention_shared", [P, L, P, P, P, I, I, P, I, P, I, I, P, P, P, P, I, I, I, I, I, I, I, ctypes.c_float, P, L, P, I, P, P])
+    for scratch in (None, 4, 8, 20):
+        for hd in (64, 20):
+            launches = I(7)
+            assert fn(16, 4 * hd, 16, 16, 16, 3, 64, None, 20000, None, 2, 1, None, None, None, None, 2, 1, 20030, 4, 2, hd, 0, 0.1, scratch, 1 << 30,
+                      16, 1, ctypes.byref(launches), None) == 1
+            assert launches.value == 0
+
+
 def floats_of(rows, n_seqs, max_q, max_kv, prefix, nq, nkv, hd, page=64, window=0, dtype=1):
     fam = family("attention_shared")
     fn = fam.declare("attention_shared_floats", [I] * 11, ctypes.c_longlong)
