@@ -1224,6 +1224,7 @@ int launch_rows(const SharedArgs& p, cudaStream_t stream) {
 FR_EXPORT long long attention_shared_floats(int rows, int n_seqs, int max_q_len, int max_kv_len, int prefix, int nq, int nkv, int hd,
                                             int page, int window, int dtype) {
     if (rows <= 0 || n_seqs <= 0 || nq <= 0 || nkv <= 0 || nq < nkv || hd <= 0) return 0;
+    if (max_q_len > rows) max_q_len = rows;
     const long long by_rows = floats_of(plan_rows(rows, nq, max_kv_len, window), rows, nq, hd);
     const TileKind kind = kind_of(rows, max_q_len, nq, nkv, hd, page, dtype);
     if (kind.rows == 0) return by_rows;
@@ -1246,6 +1247,7 @@ FR_EXPORT int attention_shared(const void* q, long long q_stride, void* out, con
     if (prefix < 0 || page < 1 || pool_pages < 1 || table_width < 0 || window < 0)
         FR_REFUSE("attention_shared: prefix %d, pages of %d, %d of them, a table %d wide, window %d", prefix, page, pool_pages, table_width, window);
     if (!(scale > 0.f) || !(scale < INFINITY)) FR_REFUSE("attention_shared: a scale of %g", (double)scale);
+    if (max_q_len > rows) max_q_len = rows;                            // (a bound may be far above what there is)
     if (rows == 1) q_stride = (long long)nq * hd;                      // (of a lone row it is never used)
     SharedArgs p = {};
     p.q = q; p.out = out; p.k_pool = k_pool; p.v_pool = v_pool; p.prefix_table = prefix_table; p.block_table = block_table;

@@ -425,6 +425,15 @@ def test_scores_far_apart(dtype):
     assert torch.equal(out[:, 16:], clean[:, 16:])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("most_rows,most_keys", [(1 << 30, 2), (2147483647, 2147483647), (7, 1)])
+def test_bounds_far_from_what_there_is(dtype, most_rows, most_keys):
+    """A bound on a sequence's rows far above the step's, bounds on the positions above and below them: the same results."""
+    b = sp.Batch(dtype, [1, 3, 7, 1], [1, 200, 90, 65], 300, 14, 2, 64, seed=49)
+    b.geometry.max_q_len, b.geometry.max_kv_len = most_rows, most_keys
+    b.check(b.run(ops), "bounds")
+
+
 def test_same_bits_every_time():
     for dtype in (F32, BF):
         b = sp.Batch(dtype, [1] * 9 + [30], [40 * i + 1 for i in range(9)] + [90], 2000, 28, 4, 128, seed=11)
