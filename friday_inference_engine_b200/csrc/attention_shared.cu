@@ -356,8 +356,9 @@ __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int
 // four stages, 16-byte asynchronous copies; what no row of the block sees, and pages that a table leaves out, come as zeros; the page
 // of a block is looked up a block before its copies are issued).  A thread has
 // the scores of up to RPT rows (4 of a warp side by side, 16 apart) with four keys, then the same rows' results in HD / 8 channels, so
-// that a row's scores, maximum and weights stay within a warp.  Bound by the multiply-adds where rows are many; a tile of few rows
-// (one token's group heads) only takes the 16-row steps that it has.
+// that a row's scores, maximum and weights stay within a warp.  Bound by what shared memory reads where rows are many; a tile of few
+// rows (one token's group heads) only takes the 16-row steps that it has.  43 rows of 5 sequences behind 1,773 keys, 16 heads on 2 of
+// 112: 40 us (66 with 4 x 4 scores per thread); 16 rows behind 4,000 keys, 28 heads on 4 of 128: 51 (81).
 namespace f32 {
 
 constexpr int KEYS = 32, THREADS = 128, LS = KEYS + 8;
@@ -463,41 +464,49 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
         int j0;
         bool own;
         range_of(i, j0, own);
-        const float* k0 = sk + i % STAGES * KEYS * LQ + tx * LQ;
+        // Four lanes (two of ty, two of tx) make the scores of all their rows with all their keys, each over every fourth group of four
+        // dimensions; then each gets the sums that are its own.  Shared memory gives a warp 128 bytes a cycle, so 8 rows x 8 keys
+        // per lane take as long to read as to multiply, where 4 x 4 take twice that: 11,800 -> 3,800 cycles a block of 128 dimensions.
+        float part[2 * N][8];
+#pragma unroll
+        for (int a = 0; a < 2 * N; ++a)
+#pragma unroll
+            for (int b = 0; b < 8; ++b) part[a][b] = 0.f;
+        const int quarter = (ty & 1) * 2 + (tx & 1);
+        const float* q0 = sq + (4 * warp + (ty & 2)) * LQ + 4 * quarter;
+        const float* k0 = sk + i % STAGES * KEYS * LQ + (tx & 6) * LQ + 4 * quarter;
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 16) {
+            float4 q[2 * N];
+#pragma unroll
+            for (int a = 0; a < 2 * N; ++a) q[a] = *(const float4*)(q0 + (16 * (a >> 1) + (a & 1)) * LQ + d);
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                const float4 k = *(const float4*)(k0 + (8 * (b >> 1) + (b & 1)) * LQ + d);
+#pragma unroll
+                for (int a = 0; a < 2 * N; ++a) part[a][b] = fmaf(q[a].x, k.x, part[a][b]);
+#pragma unroll
+                for (int a = 0; a < 2 * N; ++a) part[a][b] = fmaf(q[a].y, k.y, part[a][b]);
+#pragma unroll
+                for (int a = 0; a < 2 * N; ++a) part[a][b] = fmaf(q[a].z, k.z, part[a][b]);
+#pragma unroll
+                for (int a = 0; a < 2 * N; ++a) part[a][b] = fmaf(q[a].w, k.w, part[a][b]);
+            }
+        }
         float s[N][4];
 #pragma unroll
-        for (int a = 0; a < N; ++a)
+        for (int b = 0; b < 4; ++b) {
+            float half[2 * N];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) s[a][b] = 0.f;
-        // (sixteen dimensions at a time: the error of a score is that of short sums)
-#pragma unroll
-        for (int d0 = 0; d0 < HD; d0 += 16) {
-            float part[N][4];
-#pragma unroll
-            for (int a = 0; a < N; ++a)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) part[a][b] = 0.f;
-#pragma unroll
-            for (int d = d0; d < d0 + 16; d += 4) {
-                float4 q[N], k[4];
-#pragma unroll
-                for (int a = 0; a < N; ++a) q[a] = *(const float4*)(sq + (r0 + 16 * a) * LQ + d);
-#pragma unroll
-                for (int b = 0; b < 4; ++b) k[b] = *(const float4*)(k0 + 8 * b * LQ + d);
-#pragma unroll
-                for (int a = 0; a < N; ++a)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        part[a][b] = fmaf(q[a].x, k[b].x, part[a][b]);
-                        part[a][b] = fmaf(q[a].y, k[b].y, part[a][b]);
-                        part[a][b] = fmaf(q[a].z, k[b].z, part[a][b]);
-                        part[a][b] = fmaf(q[a].w, k[b].w, part[a][b]);
-                    }
+            for (int a = 0; a < 2 * N; ++a) {
+                const float mine = tx & 1 ? part[a][2 * b + 1] : part[a][2 * b], other = tx & 1 ? part[a][2 * b] : part[a][2 * b + 1];
+                half[a] = mine + __shfl_xor_sync(0xffffffffu, other, 1);
             }
 #pragma unroll
-            for (int a = 0; a < N; ++a)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) s[a][b] += part[a][b];
+            for (int a = 0; a < N; ++a) {
+                const float mine = ty & 1 ? half[2 * a + 1] : half[2 * a], other = ty & 1 ? half[2 * a] : half[2 * a + 1];
+                s[a][b] = mine + __shfl_xor_sync(0xffffffffu, other, 8);
+            }
         }
 #pragma unroll
         for (int a = 0; a < N; ++a) {
@@ -1138,8 +1147,8 @@ TileKind kind_of(long long rows, int max_q_len, int nq, int nkv, int hd, int pag
         k.at_once = hd <= 64 ? 3 : 2;
         const long long own = (max_q_len < k.rows / G ? max_q_len : k.rows / G) * (long long)G;
         const double steps = k.rows / 16, own_steps = own > 32 ? 4 : own > 16 ? 2 : 1, width = hd <= 32 ? 0.5 : hd <= 64 ? 1 : 2;
-        k.begin = 3.0; k.alone = width * (1.9 + 0.37 * steps); k.block = width * (1.0 + 1.2 * steps);
-        k.own_alone = width * (1.9 + 0.37 * own_steps); k.own_block = width * (1.0 + 1.2 * own_steps);
+        k.begin = 3.0; k.alone = width * (1.6 + 0.35 * steps); k.block = width * (0.9 + 0.45 * steps);
+        k.own_alone = width * (1.6 + 0.35 * own_steps); k.own_block = width * (0.9 + 0.45 * own_steps);
     }
     return k;
 }
