@@ -617,9 +617,9 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 //               swizzle), then K of the block after and V of this one (a block of 64 keys is a page); a page that a table leaves out
 //               is loaded from beyond the pool's last row, which fills zeros
 //   warp 1      tensor memory; one lane issues S = Q K^T two blocks ahead of O += P V
-//   warps 2-5   one thread per row: maximum, exponentials, running maximum and sum; P goes back into tensor memory as bf16 over its
-//               scores.  The reference maximum only moves when the true one has grown by more than 8 (in log2 units; weights stay
-//               below 2^8); O is rescaled then.
+//   warps 2-5   one thread per row: maximum, exponentials, running maximum and sum; P goes back into tensor memory (two bf16
+//               numbers a weight) over its scores.  The reference maximum only moves when the true one has grown by more than 8 (in
+//               log2 units; weights stay below 2^8); O is rescaled then.
 //
 // A CTA takes 101 KB of shared memory and half the tensor memory, so two share an SM and one's softmax runs beside the other's
 // products: 16 prompts of 2,188 rows in all behind 8,000 keys, 28 heads on 4 of 128, took 250 us this way and 288 with two tiles and
@@ -631,10 +631,16 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 // where this takes 0.68.)
 //
 // Where jobs are more than CTAs, the CTAs stay and take one job of every round, longest first: 64 one-token rows behind 16,001 keys and
-// 1 to 1,000 of their own 37 us, 48.5 with a CTA per job.  P is rounded to bf16 for the second product
-// (its sum is not); scores, sums and results are 32-bit.  Values of positions that no row of the CTA sees may be anything: their rows
-// are zeroed in shared memory before the product.  (A position that one row sees and another does not must hold finite values: zero
-// times infinity.)  Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their
+// 1 to 1,000 of their own 37 us, 48.5 with a CTA per job (both with weights of one bf16 number, see below).
+//
+// Scores, sums, weights and results are 32-bit in effect: P enters the second product as two bf16 numbers, the weight rounded over the
+// first half of its scores' columns and what rounding left over the second half, each with the same values.  One number alone was off by
+// as much again as the result's own rounding (norm of the error against 64 bits 0.0023 of the result's, 0.0017 with two), and which
+// precision a caller got went by page size and alignment; the second product takes twice its time for it: on one card 48 us for 41 (64
+// one-token rows behind 16,001), 333 for 273 (the prompts).
+//
+// Values of positions that no row of the CTA sees may be anything: their rows are zeroed in shared memory before the product.
+// (A position that one row sees and another does not must hold finite values: zero times infinity.)  Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their
 // loops.
 namespace tcore {
 
@@ -858,6 +864,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 uint32_t pa = tmem + KEYS * b, keep = i > 0 ? 1u : 0u;
                 for (int ks = 0; ks < steps; ++ks) {
                     mma_ta(tmem + 2 * KEYS, pa, db, idesc_pv, keep);
+                    mma_ta(tmem + 2 * KEYS, pa + KEYS / 2, db, idesc_pv, 1u);
                     keep = 1u;
                     pa += 8;                                   // 16 keys of P: 8 columns
                     db += (uint64_t)(16 * 128 >> 4);           // 16 keys of V
@@ -944,16 +951,22 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 unsigned long long sum2[2] = {0ull, 0ull};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {                  // (a half is on its way while the other is made)
-                    uint32_t packed[16];
+                    uint32_t head[16], rest[16];
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
                         float x0, x1;
                         halves(fma2(two(__uint_as_float(raw[32 * h + j]), __uint_as_float(raw[32 * h + j + 1])), scale2, neg2), x0, x1);
                         const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
                         sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], two(e0, e1));
-                        packed[j >> 1] = pack2(e0, e1);
+                        // a weight is two bf16 numbers: itself rounded, and what rounding left (its last 2^-16 is lost)
+                        const uint32_t w = pack2(e0, e1);
+                        float r0, r1;
+                        halves(fma2(two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), two(-1.f, -1.f), two(e0, e1)), r0, r1);
+                        head[j >> 1] = w;
+                        rest[j >> 1] = pack2(r0, r1);
                     }
-                    st16(t_s + 16 * h, packed);
+                    st16(t_s + 16 * h, head);
+                    st16(t_s + KEYS / 2 + 16 * h, rest);
                 }
                 float sum4[4];
                 halves(sum2[0], sum4[0], sum4[1]);
