@@ -226,10 +226,11 @@ __global__ void __launch_bounds__(VEC == 4 ? 128 : 256) merge_kernel(const Share
 //   own      rows of one sequence, a share of its own blocks                        -> a part
 //   whole    rows of one sequence, all of the prefix' blocks and then its own       -> the result (many rows per sequence)
 
-// a row's position, no further than the tables have room; -1: it sees nothing
-__device__ __forceinline__ int position_of(const SharedArgs& p, int row) {
+// the last position that a row at `pos` sees: its own, no further than the tables have room; -1: it sees nothing.  (Its window ends at
+// its own position, wherever the tables end: the first position that it sees goes by `pos`, and may lie behind the last.)
+__device__ __forceinline__ int last_seen(const SharedArgs& p, int pos) {
     const long long room = (long long)p.prefix + (long long)p.table_width * p.page;
-    return max(-1, (int)min((long long)p.row_pos[row], room - 1));
+    return max(-1, (int)min((long long)pos, room - 1));
 }
 
 // Keys [lo, hi] of a range of pages that the CTA's rows see between them (none: hi < lo), block `first` its first one here, n blocks.
@@ -317,14 +318,17 @@ __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int
     } else {
         int least = 0x7fffffff, most = -1;
         if (job.n_tok == 1) {                                      // (a one-token step: every thread looks for itself)
-            const int of = p.row_seq[job.row0], pos = position_of(p, job.row0);
-            if (of >= 0 && of < p.n_seqs) least = most = pos;
+            const int of = p.row_seq[job.row0], pos = p.row_pos[job.row0];
+            if (of >= 0 && of < p.n_seqs) {
+                least = pos;
+                most = last_seen(p, pos);
+            }
         } else {
             for (int t = threadIdx.x; t < job.n_tok; t += threads) {
-                const int of = p.row_seq[job.row0 + t], pos = position_of(p, job.row0 + t);
+                const int of = p.row_seq[job.row0 + t], pos = p.row_pos[job.row0 + t];
                 if (of >= 0 && of < p.n_seqs) {
                     atomicMin(&s_pos[0], pos);
-                    atomicMax(&s_pos[1], pos);
+                    atomicMax(&s_pos[1], last_seen(p, pos));
                 }
             }
             __syncthreads();
@@ -447,12 +451,15 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
         const int r = r0 + 16 * i;
         live[i] = r < n_rows;
         pos[i] = -1;
+        first[i] = 0;
         if (live[i]) {
             const int row = job.row0 + p.by_group(r), of = p.row_seq[row];
             live[i] = of >= 0 && of < p.n_seqs;
-            if (live[i]) pos[i] = position_of(p, row);
+            if (live[i]) {
+                first[i] = fr_first_key(p.row_pos[row], p.window, 0);
+                pos[i] = last_seen(p, p.row_pos[row]);
+            }
         }
-        first[i] = fr_first_key(pos[i], p.window, 0);
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
@@ -640,8 +647,8 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 // one-token rows behind 16,001), 333 for 273 (the prompts).
 //
 // Values of positions that no row of the CTA sees may be anything: their rows are zeroed in shared memory before the product.
-// (A position that one row sees and another does not must hold finite values: zero times infinity.)  Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their
-// loops.
+// (A position that one row sees and another does not must hold finite values: zero times infinity.)  Every wait on an mbarrier is
+// bounded; a wait that gives up leaves a code in `status` and all roles leave their loops.
 namespace tcore {
 
 using namespace tc;
@@ -879,14 +886,16 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         const int quarter = warp & 3;                          // the tensor-memory lanes that this warp may touch: 32 * quarter ..
         const int r = quarter * 32 + lane, t = p.by_group(r), g = r - t * G;
         const int row = row0 + t;
-        int pos = -1;
+        int pos = -1, first = 0;                               // the last and the first position that the row sees
         bool live = r < T * G && t < n_tok;
         if (live) {
             const int of = p.row_seq[row];
             live = of >= 0 && of < p.n_seqs;
-            if (live) pos = position_of(p, row);
+            if (live) {
+                first = fr_first_key(p.row_pos[row], p.window, 0);
+                pos = last_seen(p, p.row_pos[row]);
+            }
         }
-        const int first = fr_first_key(pos, p.window, 0);
         const bool any = __any_sync(0xffffffffu, live);        // a warp without rows only keeps the barriers going
         int prefix_hi = seg0.hi;                               // the last prefix position that a row of the CTA sees
         if (job.early) {
