@@ -240,6 +240,8 @@ struct Range {
 struct Job {
     int kvh, seq, row0, n_tok, part;      // n_tok token rows from row0 on
     Range seg0, seg1;                     // of the prefix; of own keys, numbered from the prefix' end
+    int all_lo, all_hi;                   // positions that every row sees that sees any; in between them others may see more
+    bool uneven;                          // there are positions that some rows see and others do not, or none between the rows' windows
     bool early;
     int first_page;                       // of own keys, looked up while the rows' positions are on the way (-2: not looked up)
 };
@@ -313,33 +315,35 @@ __device__ __forceinline__ Job job_of(const SharedArgs& p, int index, int T, int
     }
     job.seg0 = job.seg1 = Range{0, -1, 0, 0};
     job.early = early && prefix_job && p.window == 0;
+    job.all_lo = job.all_hi = 0;
+    job.uneven = false;
     if (job.early) {
         job.seg0.hi = p.prefix - 1;
     } else {
-        int least = 0x7fffffff, most = -1;
+        int least = 0x7fffffff, most = -1;                         // of the rows' positions
         if (job.n_tok == 1) {                                      // (a one-token step: every thread looks for itself)
             const int of = p.row_seq[job.row0], pos = p.row_pos[job.row0];
-            if (of >= 0 && of < p.n_seqs) {
-                least = pos;
-                most = last_seen(p, pos);
-            }
+            if (of >= 0 && of < p.n_seqs && pos >= 0) least = most = pos;
         } else {
             for (int t = threadIdx.x; t < job.n_tok; t += threads) {
                 const int of = p.row_seq[job.row0 + t], pos = p.row_pos[job.row0 + t];
-                if (of >= 0 && of < p.n_seqs) {
+                if (of >= 0 && of < p.n_seqs && pos >= 0) {
                     atomicMin(&s_pos[0], pos);
-                    atomicMax(&s_pos[1], last_seen(p, pos));
+                    atomicMax(&s_pos[1], pos);
                 }
             }
             __syncthreads();
             least = s_pos[0];
             most = s_pos[1];
         }
-        const int lo = most < 0 ? 0 : fr_first_key(least, p.window, 0);
+        const int lo = most < 0 ? 0 : fr_first_key(least, p.window, 0), hi = last_seen(p, most);
         job.seg0.lo = lo;
         job.seg1.lo = max(0, lo - p.prefix);
-        if (p.whole || prefix_job) job.seg0.hi = min(most, p.prefix - 1);
-        if (!prefix_job) job.seg1.hi = most - p.prefix;
+        if (p.whole || prefix_job) job.seg0.hi = min(hi, p.prefix - 1);
+        if (!prefix_job) job.seg1.hi = hi - p.prefix;
+        job.all_lo = fr_first_key(most, p.window, 0);
+        job.all_hi = last_seen(p, least);
+        job.uneven = most >= 0 && (lo < job.all_lo || job.all_hi < hi);
     }
     // equal shares of the blocks, the first ones a block longer where they do not come out even
     const FrDivide& shares = prefix_job ? p.by_prefix_splits : p.by_own_splits;
@@ -546,25 +550,34 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
         }
         __syncwarp();
         const float* v0 = sv + i % STAGES * KEYS * HD + 4 * tx;
+        auto results = [&](auto choosy) {
 #pragma unroll 2
-        for (int j = 0; j < KEYS; j += 4) {
-            float w[N][4];
+            for (int j = 0; j < KEYS; j += 4) {
+                float w[N][4];
 #pragma unroll
-            for (int a = 0; a < N; ++a) *(float4*)w[a] = *(const float4*)(sp + (r0 + 16 * a) * LS + j);
+                for (int a = 0; a < N; ++a) *(float4*)w[a] = *(const float4*)(sp + (r0 + 16 * a) * LS + j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+                for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const float4 v = *(const float4*)(v0 + (j + e) * HD + 32 * c);
+                    for (int c = 0; c < CH; ++c) {
+                        const float4 v = *(const float4*)(v0 + (j + e) * HD + 32 * c);
 #pragma unroll
-                    for (int a = 0; a < N; ++a) {
-                        acc[a][4 * c] = fmaf(w[a][e], v.x, acc[a][4 * c]);
-                        acc[a][4 * c + 1] = fmaf(w[a][e], v.y, acc[a][4 * c + 1]);
-                        acc[a][4 * c + 2] = fmaf(w[a][e], v.z, acc[a][4 * c + 2]);
-                        acc[a][4 * c + 3] = fmaf(w[a][e], v.w, acc[a][4 * c + 3]);
+                        for (int a = 0; a < N; ++a) {
+                            if (decltype(choosy)::value && w[a][e] == 0.f) continue;
+                            acc[a][4 * c] = fmaf(w[a][e], v.x, acc[a][4 * c]);
+                            acc[a][4 * c + 1] = fmaf(w[a][e], v.y, acc[a][4 * c + 1]);
+                            acc[a][4 * c + 2] = fmaf(w[a][e], v.z, acc[a][4 * c + 2]);
+                            acc[a][4 * c + 3] = fmaf(w[a][e], v.w, acc[a][4 * c + 3]);
+                        }
                     }
-                }
-        }
+            }
+        };
+        // (where some rows see positions that others do not: a value that a row does not see may be anything, and zero times infinity is
+        // not zero)
+        const Range& g = own ? job.seg1 : job.seg0;
+        const int seen_from = max(j0, g.lo) + (own ? p.prefix : 0), seen_to = min(j0 + KEYS - 1, g.hi) + (own ? p.prefix : 0);
+        if (job.uneven && (seen_from < job.all_lo || seen_to > job.all_hi)) results(std::true_type{});
+        else results(std::false_type{});
         __syncwarp();
     };
     const int steps = (n_rows - 4 * warp + 15) / 16;                   // 16-row steps in which this warp has rows
@@ -583,7 +596,10 @@ __global__ void __launch_bounds__(THREADS) tiles_kernel(const SharedArgs p) {
         if (!live[a]) continue;
         const int r = r0 + 16 * a, t = p.by_group(r);
         const size_t item = (size_t)(job.row0 + t) * p.nq + (size_t)job.kvh * G + r - t * G, at = item * p.parts + job.part;
-        const float inv = l[a] > 0.f ? 1.f / l[a] : l[a];              // (nothing seen: 0; a NaN stays one)
+        const float inv = l[a] > 0.f ? 1.f / l[a] : l[a];              // (a NaN stays one)
+        if (p.whole && l[a] == 0.f)                                    // nothing seen: 0, whatever was multiplied by 0
+#pragma unroll
+            for (int c = 0; c < 4 * CH; ++c) acc[a][c] = 0.f;
         float* to = p.whole ? (float*)p.out + item * p.hd : p.part + at * p.hd;
         if (!p.whole && tx == 0) *(float2*)(p.stat + 2 * at) = make_float2(m[a], l[a]);
 #pragma unroll
@@ -643,12 +659,16 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 // Scores, sums, weights and results are 32-bit in effect: P enters the second product as two bf16 numbers, the weight rounded over the
 // first half of its scores' columns and what rounding left over the second half, each with the same values.  One number alone was off by
 // as much again as the result's own rounding (norm of the error against 64 bits 0.0023 of the result's, 0.0017 with two), and which
-// precision a caller got went by page size and alignment; the second product takes twice its time for it: on one card 48 us for 41 (64
+// precision a caller got went by page size and alignment; the second product takes twice its time for it: on one card 46 us for 41 (64
 // one-token rows behind 16,001), 333 for 273 (the prompts).
 //
-// Values of positions that no row of the CTA sees may be anything: their rows are zeroed in shared memory before the product.
-// (A position that one row sees and another does not must hold finite values: zero times infinity.)  Every wait on an mbarrier is
-// bounded; a wait that gives up leaves a code in `status` and all roles leave their loops.
+// A row's result depends on nothing that it does not see.  Weights there are 0, but zero times infinity is not: in blocks that all rows of
+// the CTA see alike, values of positions that none sees are zeroed in shared memory before the product; in blocks where rows see different
+// ranges (the last ones of a prompt's tile, the edges of windows, a prefix with rows inside it) all values that are not finite are taken
+// out, and a row that sees one gets it at its end, for which those blocks' pages are read again (prompts 336 us for 333).  A row that gives
+// a weight to a value that is not finite has no finite number there.
+//
+// Every wait on an mbarrier is bounded; a wait that gives up leaves a code in `status` and all roles leave their loops.
 namespace tcore {
 
 using namespace tc;
@@ -730,6 +750,13 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+// two bf16 numbers: whether one is infinite or NaN; such ones replaced by zeros
+__device__ __forceinline__ bool not_finite(uint32_t two_numbers) {
+    return (two_numbers & 0x7f80u) == 0x7f80u || (two_numbers & 0x7f800000u) == 0x7f800000u;
+}
+__device__ __forceinline__ uint32_t finite_of(uint32_t two_numbers) {
+    return ((two_numbers & 0x7f80u) == 0x7f80u ? 0u : two_numbers & 0xffffu) | ((two_numbers & 0x7f800000u) == 0x7f800000u ? 0u : two_numbers & 0xffff0000u);
+}
 // D[tmem] (+)= A[tmem] * B[smem]: lane = row, two bf16 per column of A
 __device__ __forceinline__ void mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -750,7 +777,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     uint64_t* bars = (uint64_t*)(s_v + 2 * STAGE);
     // bars: q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2]
     uint32_t* tmem_slot = (uint32_t*)(bars + 15);
-    int* s_pos = (int*)(tmem_slot + 1);               // a wait gave up; least, greatest position of a live row, for even and odd rounds; then room for order_by_length
+    // a wait gave up; least, greatest position of a live row, for even and odd rounds; room for order_by_length; values were taken out, for
+    // even and odd rounds
+    int* s_pos = (int*)(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t q_full = smem_u32(bars), k_full = smem_u32(bars + 1), k_empty = smem_u32(bars + 3);
@@ -771,6 +800,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         s_pos[0] = 0;
         s_pos[1] = s_pos[3] = 0x7fffffff;
         s_pos[2] = s_pos[4] = -1;
+        s_pos[5 + 2 * THREADS] = s_pos[6 + 2 * THREADS] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -801,6 +831,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if ((long long)round * gridDim.x >= p.jobs) break;
     if (index >= p.jobs) continue;
     int* const s_range = s_pos + 1 + 2 * (round & 1);
+    volatile int* const s_taken = s_pos + 5 + 2 * THREADS + (round & 1);
     const Job job = job_of<KEYS, THREADS>(p, (int)index, T, s_range, s_order, true);
     const Range seg0 = job.seg0, seg1 = job.seg1;
     const int kvh = job.kvh, seq = job.seq, row0 = job.row0, n_tok = job.n_tok, part = job.part;
@@ -898,11 +929,29 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         const bool any = __any_sync(0xffffffffu, live);        // a warp without rows only keeps the barriers going
         int prefix_hi = seg0.hi;                               // the last prefix position that a row of the CTA sees
+        int all_lo = job.all_lo, all_hi = job.all_hi;
+        bool uneven = job.uneven;
         if (job.early) {
-            if (live) atomicMax(&s_range[1], pos);
+            if (live && pos >= 0) {
+                atomicMin(&s_range[0], pos);
+                atomicMax(&s_range[1], pos);
+            }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             prefix_hi = min(seg0.hi, s_range[1]);
+            all_lo = 0;
+            all_hi = s_range[0];
+            uneven = all_hi < prefix_hi;
         }
+        // Whether some row sees a position of block i that another does not: of each range the blocks but [from, to) are mixed.
+        int even_from0 = 0, even_to0 = seg0.n, even_from1 = seg0.n, even_to1 = n_blocks;
+        if (uneven) {
+            const int lo0 = all_lo, hi0 = all_hi, lo1 = all_lo - p.prefix, hi1 = all_hi - p.prefix;          // in each range's numbers
+            if (seg0.lo < lo0) even_from0 = (int)(((unsigned)lo0 + KEYS - 1) / KEYS) - seg0.first;
+            if (prefix_hi > hi0) even_to0 = max(hi0 + 1, 0) / KEYS - seg0.first;
+            if (seg1.lo < lo1) even_from1 = seg0.n + (int)(((unsigned)lo1 + KEYS - 1) / KEYS) - seg1.first;
+            if (seg1.hi > hi1) even_to1 = seg0.n + max(hi1 + 1, 0) / KEYS - seg1.first;
+        }
+        auto mixed = [&](int i) { return i < seg0.n ? i < even_from0 || i >= even_to0 : i < even_from1 || i >= even_to1; };
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16, t_o = tmem + lane_addr + 2 * KEYS;
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
@@ -984,7 +1033,26 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 st_wait();
             }
             const int in_lo = (own ? seg1.lo : seg0.lo) - j0, in_hi = (own ? seg1.hi : prefix_hi) - j0;
-            if (in_lo > 0 || in_hi < KEYS - 1) {
+            if (mixed(i)) {
+                // Values that are not finite are taken out (zero times infinity is not zero); rows that see them get them at the end.
+                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 7))) break;
+                bool found = false;
+                for (int s = 0; s < slices; ++s) {
+                    // (a row's eight pieces of 16 bytes shared by two threads, lanes in different banks)
+                    uint32_t* line = (uint32_t*)(s_v + b * STAGE + s * KSLICE + (r & (KEYS - 1)) * 128);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint4* const at = (uint4*)line + ((r + (r / KEYS) * 4 + q) & 7);
+                        uint4 v = *at;
+                        if (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) {
+                            found = true;
+                            *at = make_uint4(finite_of(v.x), finite_of(v.y), finite_of(v.z), finite_of(v.w));
+                        }
+                    }
+                }
+                if (found) *s_taken = 1;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            } else if (in_lo > 0 || in_hi < KEYS - 1) {
                 // positions that no row of the CTA sees: their values may be anything
                 if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 7))) break;
                 if (r < KEYS && (r < in_lo || r > in_hi)) {
@@ -1004,6 +1072,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             tc_fence_after();
         }
         if (!ok) s_pos[0] = 1;
+        if (uneven) asm volatile("bar.sync 1, 128;" ::: "memory");          // (s_taken is everyone's)
+        const bool taken = uneven && *s_taken != 0;
         if (ok && any) {
             const size_t item = (size_t)row * p.nq + (size_t)kvh * G + g;
             const bool seen = l_run != 0.f;                    // (a NaN is seen)
@@ -1035,6 +1105,34 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     for (int j = 0; j < 16; j += 4) *(uint4*)(line + (c + j) * 4) = make_uint4(o16[j], o16[j + 1], o16[j + 2], o16[j + 3]);
                 }
             }
+            if (taken && live && seen) {
+                // what was taken out of the values, for a row that sees it: its number is no longer finite
+#pragma unroll 1
+                for (int i = 0; i < n_blocks; ++i) {
+                    if (!mixed(i)) continue;
+                    const bool own = i >= seg0.n;
+                    const int from = first_key_of(i) + (own ? p.prefix : 0), to = min(from + KEYS - 1, own ? pos : min(pos, p.prefix - 1));
+#pragma unroll 1
+                    for (int j = max(from, first); j <= to; ++j) {
+                        const long long place = place_of(p, seq, j);
+                        if (place < 0) continue;
+                        const bf16* value = (const bf16*)p.v_pool + ((size_t)place * p.nkv + kvh) * p.hd;
+#pragma unroll 2
+                        for (int c = 0; c < p.hd; c += 8) {
+                            const uint4 v = *(const uint4*)(value + c);
+                            if (!(not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w))) continue;
+#pragma unroll 1
+                            for (int e = c; e < c + 8; ++e) {
+                                const float one = __bfloat162float(value[e]);
+                                if (fabsf(one) < INFINITY) continue;
+                                bf16* const result = (bf16*)p.out + item * p.hd + e;
+                                if (p.whole) *result = __float2bfloat16_rn(__bfloat162float(*result) + one);
+                                else ((float*)line)[e] += one;
+                            }
+                        }
+                    }
+                }
+            }
             if (!p.whole && live && seen) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.part + at * p.hd), "r"(smem_u32(line)),
@@ -1052,6 +1150,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         // the next round's pair of positions, which nobody has read since the round before this one
         s_pos[1 + 2 * (round + 1 & 1)] = 0x7fffffff;
         s_pos[2 + 2 * (round + 1 & 1)] = -1;
+        s_pos[5 + 2 * THREADS + (round + 1 & 1)] = 0;
     }
     tc_fence_before();
     __syncthreads();

@@ -426,9 +426,9 @@ public:
     // Attention of the step's rows where every sequence begins with the same prefix_len positions: those keys and values lie in the
     // pages of prefix_table (device), a sequence's further ones in its row of the view's block table, from the first page on.  A row
     // at position p sees position j if p - window < j <= p (window 0: every j <= p); one that sees nothing gives zeros; one whose
-    // row_seq is negative is not written.  Pages that a table leaves out read as zeros; positions that no row sees may hold anything,
-    // values of those that some row sees are finite.  The rows of sequence s are ctx.seq_start[s]
-    // and the seq_qlen[s] - 1 after it; ctx.max_kv_len bounds the positions (prefix included) and only shares the work out.
+    // row_seq is negative is not written.  Pages that a table leaves out read as zeros.  A row's result depends on nothing that the
+    // row does not see; one that gives a weight to a value that is not finite has no finite number there.  The rows of sequence s are
+    // ctx.seq_start[s] and the seq_qlen[s] - 1 after it; ctx.max_kv_len bounds the positions (prefix included) and only shares the work out.
     // Prefix and own keys are read once for all rows that share them.  prefix_len is the host's: a captured call keeps it.
     void attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const CacheView& view, const int* prefix_table, int prefix_len,
                           const StepContext& ctx, int n_heads, int n_kv_heads, int head_dim, int window, float scale,

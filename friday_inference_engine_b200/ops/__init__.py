@@ -302,8 +302,8 @@ class CudaOps:
         prefix_table (int32, may be None without a prefix); block_table [sequences, pages] names each sequence's own pages, its
         position prefix_len being the first row of the first of them.  A row at position p (row_pos, prefix included) sees position j
         if p - window < j <= p (window 0 or None: every j <= p) and a table has room for it; a page that a table leaves out reads as
-        zeros.  A row that sees nothing gives zeros; a row whose row_seq is negative is not written.  Values of positions that some row
-        sees must be finite.
+        zeros.  A row that sees nothing gives zeros; a row whose row_seq is negative is not written.  A row's result depends on
+        nothing that the row does not see; one that gives a weight to a value that is not finite has no finite number there.
 
         geometry: an object with n_seqs, max_q_len, max_kv_len (prefix included) and the arrays seq_start and seq_qlen (int32,
         device): the rows of sequence s are seq_start[s] and the seq_qlen[s] - 1 after it, row_seq says so too.  max_q_len bounds

@@ -60,3 +60,73 @@ def test_windows_of_rows_behind_the_tables_end(dtype, heads, kv_heads, hd, q_len
     c = copy.copy(b)                                      # (the definition, for the others)
     c.row_seq = torch.where(nothing, -1, b.row_seq)
     c.check(torch.where(nothing[:, None], 7.25, out.float()).to(dtype), "windows behind the tables' end")
+
+
+# ------------------------------------------------------------------ values that a row does not see
+def seen_places(b):
+    """(prefix positions [rows, prefix], own positions [rows, own pages * PAGE]) that each row sees, as truth values."""
+    width = b.block_table.shape[1] * PAGE
+    j = torch.arange(b.prefix + width, device=DEV)
+    pos = b.row_pos.long()[:, None]
+    seen = (j <= pos) & (b.row_seq >= 0)[:, None]
+    if b.window > 0:
+        seen &= j > pos - b.window
+    return seen[:, :b.prefix], seen[:, b.prefix:]
+
+
+SPREAD = [  # q_lens, own_lens, prefix, window, positions of the rows (None: as they are)
+    ([1, 1], [1, 1], 600, 32, [40, 290]),                                    # two windows far apart in one tile of the prefix
+    ([1] * 6, [200] * 6, 700, 90, [3, 200, 291, 500, 760, 899]),             # some behind the prefix
+    ([2, 40], [3, 40], 500, 20, [(37 * i) % 530 for i in range(42)]),        # in no order, near the prefix' end
+    ([5, 60], [70, 300], 130, 7, list(range(130, 200, 14)) + [130 + 4 * i for i in range(60)]),        # holes among own keys
+    ([1, 30], [1, 90], 300, 0, [5] + list(range(290, 320)))]                 # no window: rows inside the prefix
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 2, 16), (28, 4, 128), (8, 8, 80), (14, 2, 64), (2, 2, 20)])
+@pytest.mark.parametrize("shape", range(len(SPREAD)))
+def test_places_that_no_row_sees_hold_anything(dtype, heads, kv_heads, hd, shape):
+    q_lens, own, prefix, window, positions = SPREAD[shape]
+    b = sp.Batch(dtype, q_lens, own, prefix, heads, kv_heads, hd, window=window, seed=90 + shape)
+    b.k_pool.nan_to_num_(0.5)
+    b.v_pool.nan_to_num_(0.25)
+    b.row_pos.copy_(torch.tensor(positions, dtype=torch.int32))
+    in_prefix, in_own = seen_places(b)
+    j = (~in_prefix.any(0)).nonzero().flatten()
+    for pool, bad in ((b.k_pool, float("nan")), (b.v_pool, float("inf"))):
+        pool[b.prefix_table.long()[j // PAGE], j % PAGE] = bad
+        for s in range(len(q_lens)):
+            k = (~in_own[b.row_seq == s].any(0)).nonzero().flatten()
+            k = k[b.block_table[s, k // PAGE] >= 0]
+            pool[b.block_table[s, k // PAGE].long(), k % PAGE] = bad
+    b.check(b.run(ops), "numbers nowhere but where a row looks")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 2, 16), (28, 4, 128), (8, 8, 80), (14, 2, 64), (2, 2, 20)])
+@pytest.mark.parametrize("shape", range(len(SPREAD)))
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(dtype, heads, kv_heads, hd, shape):
+    """A row's numbers depend on nothing that it does not see, whatever the rows of its tile see."""
+    q_lens, own, prefix, window, positions = SPREAD[shape]
+    b = sp.Batch(dtype, q_lens, own, prefix, heads, kv_heads, hd, window=window, seed=70 + shape)
+    b.k_pool.nan_to_num_(0.5)
+    b.v_pool.nan_to_num_(0.25)
+    b.row_pos.copy_(torch.tensor(positions, dtype=torch.int32))
+    clean = b.v_pool.clone()
+    in_prefix, in_own = seen_places(b)
+    spoilt = torch.zeros((len(b.row_pos), kv_heads, heads // kv_heads, hd), dtype=torch.bool, device=DEV)
+    for n, (j, kvh, c, bad) in enumerate([(38, 0, 3, "inf"), (64, kv_heads - 1, hd - 1, "nan"), (prefix - 1, 0, 5, "-inf"), (290, 0, 2, "inf"), (127, kv_heads - 1, 4, "inf")]):
+        if j < prefix:
+            b.v_pool[b.prefix_table[j // PAGE].long(), j % PAGE, kvh, c] = float(bad)
+            spoilt[:, kvh, :, c] |= in_prefix[:, j, None]
+    for s in range(len(q_lens)):
+        for k, kvh, c, bad in ((0, 0, 7, "inf"), (own[s] // 2, kv_heads - 1, 1, "nan"), (own[s] - 1, 0, 0, "inf")):
+            b.v_pool[b.block_table[s, k // PAGE].long(), k % PAGE, kvh, c] = float(bad)
+            spoilt[:, kvh, :, c] |= (in_own[:, k] & (b.row_seq == s))[:, None]
+    out = b.run(ops)
+    spoilt = spoilt.flatten(1)
+    finite = out.isfinite()
+    assert bool((finite == ~spoilt).all()), "%d numbers spoilt by what their row does not see, %d clean that should not be" % (
+        int((~finite & ~spoilt).sum()), int((finite & spoilt).sum()))
+    b.v_pool = clean                                      # (the definition without them, for all other numbers)
+    b.check(torch.where(spoilt, b.reference()[0].to(dtype), out), "numbers beside")
