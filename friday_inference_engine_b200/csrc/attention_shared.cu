@@ -848,7 +848,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             for (int s = 0; s < slices; ++s) load_4d(smem_u32(s_q + s * SLICE), &map_q, s * 64, 0, kvh, row0, q_full);
             auto load = [&](int i, const CUtensorMap* map, uint8_t* ring, uint32_t full, uint32_t empty) {
                 const int b = stage_of(i), par = parity_of(i);
-                if (!mbar_wait(empty + 8 * b, par ^ 1, p.status, 1)) return false;
+                if (!mbar_wait(empty + 8 * b, par ^ 1, p.status, 31)) return false;
                 mbar_expect_tx(full + 8 * b, (uint32_t)(slices * KSLICE));
                 const int* table = i < seg0.n ? p.prefix_table : p.block_table + (size_t)seq * p.table_width;
                 int page = i == 0 && job.first_page != -2 ? job.first_page : table[first_key_of(i) / PAGE];
@@ -869,12 +869,12 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             const uint32_t idesc_qk = instr_desc(ROWS, KEYS);
             const uint32_t idesc_pv = instr_desc(ROWS, p.hd) | (1u << 16);              // B is MN-major
             const int k_steps = p.hd / 16;
-            bool ok = mbar_wait(q_full, loads_before & 1, p.status, 2);
+            bool ok = mbar_wait(q_full, loads_before & 1, p.status, 32);
             // (descriptors are made once and stepped: a lone thread issues all of this)
             const uint64_t dq0 = smem_desc(smem_u32(s_q)), dk0 = smem_desc(smem_u32(s_k)), dv0 = desc_mn(smem_u32(s_v), KSLICE, 1024);
             auto scores = [&](int i) {
                 const int b = stage_of(i), par = parity_of(i);
-                if (!mbar_wait(k_full + 8 * b, par, p.status, 3)) return false;
+                if (!mbar_wait(k_full + 8 * b, par, p.status, 33)) return false;
                 tc_fence_after();
                 uint64_t da = dq0, db = dk0 + (uint64_t)(b * (STAGE >> 4));
                 const uint32_t d = tmem + KEYS * b;
@@ -894,8 +894,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             if (ok && n_blocks > 1) ok = scores(1);
             for (int i = 0; i < n_blocks && ok; ++i) {
                 const int b = stage_of(i), par = parity_of(i);
-                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 4))) break;
-                if (!(ok = mbar_wait(p_full + 8 * b, par, p.status, 5))) break;
+                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 34))) break;
+                if (!(ok = mbar_wait(p_full + 8 * b, par, p.status, 35))) break;
                 tc_fence_after();
                 const int steps = (min(KEYS, last_key_of(i) - first_key_of(i) + 1) + 15) / 16;
                 uint64_t db = dv0 + (uint64_t)(b * (STAGE >> 4));
@@ -959,7 +959,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             const int b = stage_of(i), par = parity_of(i);
             const bool own = i >= seg0.n;
             const int j0 = first_key_of(i);
-            if (!(ok = mbar_wait(s_full + 8 * b, par, p.status, 6))) break;
+            if (!(ok = mbar_wait(s_full + 8 * b, par, p.status, 36))) break;
             tc_fence_after();
             const uint32_t t_s = tmem + lane_addr + KEYS * b;
             if (any) {
@@ -989,7 +989,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     if (i > 0) {
                         // Every product into O so far must be done: that of block i - 2 is (this block's scores were issued behind
                         // it), so the wait for the other stage's phase is unambiguous.
-                        if (!(ok = mbar_wait(pv_done + 8 * (b ^ 1), parity_of(i - 1), p.status, 8))) break;
+                        if (!(ok = mbar_wait(pv_done + 8 * (b ^ 1), parity_of(i - 1), p.status, 38))) break;
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < p.hd; c += 16) {
@@ -1035,7 +1035,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             const int in_lo = (own ? seg1.lo : seg0.lo) - j0, in_hi = (own ? seg1.hi : prefix_hi) - j0;
             if (mixed(i)) {
                 // Values that are not finite are taken out (zero times infinity is not zero); rows that see them get them at the end.
-                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 7))) break;
+                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 37))) break;
                 bool found = false;
                 for (int s = 0; s < slices; ++s) {
                     // (a row's eight pieces of 16 bytes shared by two threads, lanes in different banks)
@@ -1054,7 +1054,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             } else if (in_lo > 0 || in_hi < KEYS - 1) {
                 // positions that no row of the CTA sees: their values may be anything
-                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 7))) break;
+                if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 37))) break;
                 if (r < KEYS && (r < in_lo || r > in_hi)) {
                     for (int s = 0; s < slices; ++s) {
                         uint4* line = (uint4*)(s_v + b * STAGE + s * KSLICE + r * 128);
@@ -1068,7 +1068,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             mbar_arrive(p_full + 8 * b);
         }
         if (ok && n_blocks > 0) {
-            ok = mbar_wait(pv_done + 8 * stage_of(n_blocks - 1), parity_of(n_blocks - 1), p.status, 8);
+            ok = mbar_wait(pv_done + 8 * stage_of(n_blocks - 1), parity_of(n_blocks - 1), p.status, 38);
             tc_fence_after();
         }
         if (!ok) s_pos[0] = 1;

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(RING_THREADS, RING_BLOCKS) rope_axes_ring_kern
         if (g >= groups) break;
         const int row0 = (int)g * un.rows, rows = min(un.rows, p.rows - row0), b = k % STAGES;
         fetch(k + 1);
-        const bool here = tc::mbar_wait(full + 8 * b, (k / STAGES) & 1, p.status, 11);
+        const bool here = tc::mbar_wait(full + 8 * b, (k / STAGES) & 1, p.status, 41);
         if (!__syncthreads_and(here)) break;                   // (a copy that never came: nothing more is sent)
         uint8_t* stage = ring + b * stage_bytes;
         const float2* table = tables + (k & 1) * un.rows * p.half;

@@ -906,3 +906,11 @@ FR_API int friday_ops_info(void* h, const char** json) {
     })
 }
 FR_API int friday_ops_check_status(void* h) { GUARD(((OpsHandle*)h)->ops->check_status()) }
+FR_API int friday_ops_check_stream(void* h, void* stream) {
+    GUARD({
+        Ops& ops = *((OpsHandle*)h)->ops;
+        OnDevice on(ops.device());
+        ops.check_status((cudaStream_t)stream);
+    })
+}
+FR_API int friday_ops_stream_status(void* h, void* stream, int** word) { GUARD(*word = ((OpsHandle*)h)->ops->status_word((cudaStream_t)stream)) }

@@ -148,8 +148,9 @@ int friday_ops_linear_swiglu(void* ops, const FridayTensor* x, const FridayTenso
 int friday_ops_attention(void* ops, const FridayTensor* q, int64_t q_stride, FridayTensor* out, const FridayKV* kv,
                          const FridayGeometry* geometry, int n_heads, int n_kv_heads, int head_dim, int window, float scale);
 /* Rotary positions with several axes, their append to the cache, attention of a batch with a shared prefix (friday::Ops::rotate_axes,
- * rope_axes_kv_write, attention_shared).  They run on the stream that is given, use nothing of the handle that another call could be
- * using, and leave the calling thread's current device as it was.  Rows are given by address, rows, columns and row length (ld);
+ * rope_axes_kv_write, attention_shared).  They run on the stream that is given, use nothing of the handle that a call on another stream
+ * could be using, and leave the calling thread's current device as it was.  A kernel whose bounded wait gave up says so in a word of its
+ * stream's: friday_ops_check_stream reads it.  Rows are given by address, rows, columns and row length (ld);
  * dtype 0 float32, 1 bfloat16; sections: host, [axes]; pools [pages][page_size][n_kv_heads][head_dim]; block_table [n_seqs][table_width];
  * results and scratch are the caller's. */
 int friday_ops_rotate_axes(void* ops, const void* x, int64_t x_rows, int64_t x_cols, int64_t x_ld, void* out, int64_t out_rows,
@@ -176,7 +177,14 @@ int friday_ops_decode_splits(void* ops, int n_seqs, int n_heads, int n_kv_heads,
 int friday_ops_attention_splits(void* ops, int64_t rows, int n_heads, int max_kv_len, int* splits);
 int friday_ops_tensor_core_ok(void* ops, const FridayTensor* x, const FridayTensor* weight, const FridayTensor* out, int* ok);
 int friday_ops_info(void* ops, const char** json);          /* sm_count, fusion, launches, status word address */
+/* An error if a kernel recorded that one of its bounded waits gave up, so that its results are not valid; the record is cleared.
+ * check_status: of the handle's own calls; waits for the handle's stream (the legacy default stream, which does not wait for streams that
+ * were made non-blocking).  check_stream: of calls that were given `stream` (rotate_axes, rope_axes_kv_write, attention_shared); waits for
+ * that stream.  Replays of a captured call report to the stream that it was captured on: wait for the replay, then ask about that stream.
+ * stream_status: the device address of a stream's word, for callers that read it themselves. */
 int friday_ops_check_status(void* ops);
+int friday_ops_check_stream(void* ops, void* stream);
+int friday_ops_stream_status(void* ops, void* stream, int** word);
 
 #ifdef __cplusplus
 }

@@ -11,6 +11,7 @@
 
 #include <map>
 #include <memory>
+#include <mutex>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -397,7 +398,8 @@ public:
     // ---- a batch whose sequences share a long prefix, and rotary positions with several axes (csrc/rope_axes.cu,
     // csrc/attention_shared.cu)
     // Where a call runs and what it works in, if not the Ops object's stream and arena: the caller's stream, and scratch that the
-    // caller keeps until the work is done.  With a Place a call touches nothing of the Ops object that another call could.
+    // caller keeps until the work is done.  With a Place a call touches nothing of the Ops object that a call on another stream could:
+    // a wait that gives up is recorded in the stream's own word, which check_status(stream) reads.
     struct Place {
         cudaStream_t stream = nullptr;
         float* scratch = nullptr;
@@ -462,6 +464,11 @@ public:
     // where the host waits for the device anyway); clears the word.
     void check_status();
     int* status_word() const { return (int*)status_.get(); }
+    // The same for calls that were given `stream` in a Place: waits for the stream's work, reads the stream's word, clears it.  A call
+    // that was captured reports to the stream that it was captured on (which is asked about once the replay's stream is done).  The
+    // first 252 streams have a word each; those after them share the Ops object's own.
+    void check_status(cudaStream_t stream);
+    int* status_word(cudaStream_t stream);
 
     // ---- for tests and measurements
     Tensor linear_tc(const Tensor& x, const Tensor& weight, const Tensor* bias, const Tensor* residual, Tensor& out,
@@ -504,6 +511,10 @@ private:
     cudaStream_t stream_;
     void* chunk_room(size_t bytes);                           // null: no memory for them now
     DeviceBuffer tc_scratch_, tc_counters_, status_, attn_counters_;
+    static constexpr size_t MOST_STREAMS = 252;
+    std::mutex streams_lock_;
+    std::vector<cudaStream_t> streams_;                       // the n-th one's status word is the n-th behind the object's own four
+    void check_word(int* word, cudaStream_t stream);
     DeviceBuffer chunks_;                                     // prepared chunks of the delta rule's prompts (one stream uses them in turn)
     std::map<std::tuple<int64_t, int64_t, int64_t>, std::tuple<bool, int, int>> plans_;
     std::map<std::pair<int, int>, int> cluster_fit_;

@@ -163,6 +163,8 @@ _SIGNATURES = {
     "friday_ops_tensor_core_ok": [P, T, T, T, PI],
     "friday_ops_info": [P, PS],
     "friday_ops_check_status": [P],
+    "friday_ops_check_stream": [P, P],
+    "friday_ops_stream_status": [P, P, PP],
 }
 _VOID = {"friday_engine_free": [P], "friday_cache_free": [P], "friday_decoder_free": [P], "friday_ops_free": [P],
          "friday_safetensors_free": [P]}

@@ -6,8 +6,10 @@ library's own CUDA kernels; nothing is computed here, and there is no CPU path.
 Kernels run on the legacy default stream, which is also torch's default, so they are
 ordered with the torch operations around them.  (rotate_axes, rope_axes_kv_write and
 attention_shared run on torch's current stream instead, may be captured into a CUDA graph
-there, and may be called from several threads at once.)
+there, and may be called from several threads at once; check_status() says of which stream's
+kernels it speaks.)
 """
+import sys
 from ctypes import byref, c_int, c_void_p
 
 from .. import native
@@ -136,8 +138,19 @@ class CudaOps:
     def info(self):
         return native.call_json("friday_ops_info", self._h)
 
-    def check_status(self):
+    def check_status(self, stream=None):
+        """Raises if a kernel recorded that one of its bounded waits gave up, so that its results are not valid, and clears the record.
+        Waits for the work of the backend's own stream, then for that of `stream` (a torch stream; None: torch's current one), whose
+        calls of rotate_axes, rope_axes_kv_write and attention_shared report to a word of that stream's: other streams' failures stay
+        for those who ask about them.  Replays of a captured call report to the stream that it was captured on; wait for the replay,
+        then ask about that stream."""
         native.call("friday_ops_check_status", self._h)
+        if stream is None:
+            torch = sys.modules.get("torch")
+            if torch is None:                             # (no torch, no streams of its)
+                return
+            stream = torch.cuda.current_stream(self.device)
+        native.call("friday_ops_check_stream", self._h, stream.cuda_stream)
 
     # -- row-wise ---------------------------------------------------------
     def embedding(self, tokens, table, out=None):

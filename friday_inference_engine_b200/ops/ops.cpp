@@ -67,7 +67,7 @@ Ops::Ops(int device, cudaStream_t stream) : device_(device), stream_(stream) {
     // the word in which a kernel records a wait that gave up: made once, so that captured graphs keep their addresses.
     tc_scratch_ = DeviceBuffer((size_t)2 * sms_ * 128 * 256 * sizeof(float));
     tc_counters_ = DeviceBuffer(4096 * sizeof(int), true);
-    status_ = DeviceBuffer(4 * sizeof(int), true);
+    status_ = DeviceBuffer((4 + MOST_STREAMS) * sizeof(int), true);
     attn_counters_ = DeviceBuffer(((size_t)1 << 16) * sizeof(int), true);
     attn_tc_ = env_on("FRIDAY_ATTN_TC");
     profile_ = env_on("FRIDAY_PROFILE", false);
@@ -1756,7 +1756,8 @@ void Ops::rotate_axes(const Tensor& x, Tensor& out, const int* positions, const 
     const auto& k = kernels::rope_axes();
     std::unique_ptr<Timed> t(place ? nullptr : new Timed(*this, Other));
     const int rc = k.rotate(x.data, x.ld, out.data, out.ld, (int)x.rows(), heads, head_dim, positions, (int)spec.sections.size(), spec.denominators,
-                            spec.sections.data(), spec.interleaved, spec.neighbours, (int*)status_.get(), code(x.dtype), place ? place->stream : stream_);
+                            spec.sections.data(), spec.interleaved, spec.neighbours, place ? status_word(place->stream) : status_word(), code(x.dtype),
+                            place ? place->stream : stream_);
     if (rc != 0) throw KernelError(std::string("rotate_axes: ") + k.last_error());
     __atomic_add_fetch(&launches_, x.rows() > 0 ? 1 : 0, __ATOMIC_RELAXED);
 }
@@ -1788,7 +1789,7 @@ void Ops::rope_axes_kv_write(const Tensor& qkv, Tensor* q_out, const int* row_se
     const int rc = k.append(qkv.data, qkv.ld, n_heads > 0 ? q_out->data : nullptr, n_heads > 0 ? q_out->ld : 0, (int)qkv.rows(), n_heads, n_kv_heads,
                             head_dim, row_seq, row_pos, positions, (int)spec.sections.size(), spec.denominators, spec.sections.data(),
                             spec.interleaved, spec.neighbours, view.k_pool, view.v_pool, view.pool_pages, view.page_size, view.block_table,
-                            n_seqs, view.table_width, (int*)status_.get(), code(qkv.dtype), place ? place->stream : stream_);
+                            n_seqs, view.table_width, place ? status_word(place->stream) : status_word(), code(qkv.dtype), place ? place->stream : stream_);
     if (rc != 0) throw KernelError(std::string("rope_axes_kv_write: ") + k.last_error());
     __atomic_add_fetch(&launches_, qkv.rows() > 0 ? 1 : 0, __ATOMIC_RELAXED);
 }
@@ -1829,7 +1830,8 @@ void Ops::attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const
     int launches = 0;
     const int rc = k.run(q.data, q_stride, out.data, view.k_pool, view.v_pool, view.pool_pages, view.page_size, prefix_table, prefix_len, view.block_table,
                          ctx.n_seqs, view.table_width, ctx.row_seq, ctx.row_pos, ctx.seq_start, ctx.seq_qlen, rows, ctx.max_q_len, ctx.max_kv_len, n_heads,
-                         n_kv_heads, head_dim, window, scale, scratch, floats, (int*)status_.get(), code(out.dtype), &launches, place ? place->stream : stream_);
+                         n_kv_heads, head_dim, window, scale, scratch, floats, place ? status_word(place->stream) : status_word(), code(out.dtype),
+                         &launches, place ? place->stream : stream_);
     if (rc != 0) throw KernelError(std::string("attention_shared: ") + k.last_error());
     __atomic_add_fetch(&launches_, launches, __ATOMIC_RELAXED);
 }
@@ -1846,15 +1848,37 @@ void Ops::sample(const Tensor& logits, const float* temperature, const int* stre
          "sampling_sample");
 }
 
-void Ops::check_status() {
-    int word[4] = {0, 0, 0, 0};
-    cuda_check(cudaMemcpyAsync(word, status_.get(), sizeof word, cudaMemcpyDeviceToHost, stream_), "cudaMemcpyAsync");
-    cuda_check(cudaStreamSynchronize(stream_), "cudaStreamSynchronize");
-    if (word[0] != 0) {
-        cuda_check(cudaMemsetAsync(status_.get(), 0, sizeof word, stream_), "cudaMemsetAsync");
-        throw KernelError(format("a tensor-core kernel on device %d gave up waiting (code %d: which of its bounded waits, "
-                                 "see gemm_tc.cu and attention_tc.cu); its results are not valid", device_, word[0]));
+// ------------------------------------------------------------------ waits that gave up
+int* Ops::status_word(cudaStream_t stream) {
+    int* const own = status_word();
+    if (stream == stream_) return own;
+    std::lock_guard<std::mutex> lock(streams_lock_);
+    size_t n = 0;
+    while (n < streams_.size() && streams_[n] != stream) ++n;
+    if (n == MOST_STREAMS) return own;
+    if (n == streams_.size()) streams_.push_back(stream);
+    return own + 4 + n;
+}
+
+void Ops::check_word(int* word, cudaStream_t stream) {
+    int code = 0;
+    cuda_check(cudaMemcpyAsync(&code, word, sizeof code, cudaMemcpyDeviceToHost, stream), "cudaMemcpyAsync");
+    cuda_check(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
+    if (code != 0) {
+        cuda_check(cudaMemsetAsync(word, 0, sizeof code, stream), "cudaMemsetAsync");
+        throw KernelError(format("a kernel on device %d gave up waiting (code %d: which of its bounded waits; 1 to 8 gemm_tc.cu and attention_tc.cu, "
+                                 "11 to 19 gemm_f32_tc.cuh, 21 and 22 attention_mma.cu, 31 to 38 attention_shared.cu, 41 rope_axes.cu); its results "
+                                 "are not valid", device_, code));
     }
+}
+
+void Ops::check_status() { check_word(status_word(), stream_); }
+
+void Ops::check_status(cudaStream_t stream) {
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (stream != stream_ && cudaStreamIsCapturing(stream, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone)
+        throw KernelError("a stream cannot be asked about kernels that gave up while it is being captured");
+    check_word(status_word(stream), stream);
 }
 
 }  // namespace friday
