@@ -16,7 +16,7 @@ per-user folder under the system's temporary directory.
     python -m friday_inference_engine_b200.ops.build        # everything, for C++ users
 
 One file more is for Python alone: binding/torch_ops.cpp becomes friday_torch_ops.so, an extension module made against the
-installed torch (the operators whose calls must cost little).
+installed torch (the operators whose calls must cost little).  Where there is no torch, everything else is built all the same.
 
 There is no fallback: a library that cannot be built or loaded raises.
 """
@@ -316,8 +316,25 @@ def _binding_fingerprint():
     return h.hexdigest()
 
 
+def binding_lacks():
+    """What the extension module would need here and does not find (None: nothing).  The libraries need none of it."""
+    import sysconfig
+    try:
+        import torch
+    except ImportError:
+        return "torch cannot be imported"
+    if torch.version.cuda is None:
+        return "torch is built without CUDA"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers are not installed"
+    return None
+
+
 def ensure_binding_built(progress=True):
     """Compiles binding/torch_ops.cpp unless the module was made from the present source, for this torch and this Python."""
+    lacks = binding_lacks()
+    if lacks is not None:
+        raise BuildError("the binding for torch tensors cannot be built: %s" % lacks)
     with _binding_lock:
         lib, want = binding_path(), _binding_fingerprint()
         try:
@@ -346,7 +363,13 @@ def build_all(progress=True):
     fams = [f for f in FAMILIES if os.path.exists(os.path.join(CSRC, f + ".cu"))]
     engine = ensure_engine_built(progress=progress)
     ensure_built(fams, progress=progress)
-    return [engine] + [library_path(f) for f in fams] + [ensure_binding_built(progress=progress)]
+    made = [engine] + [library_path(f) for f in fams]
+    lacks = binding_lacks()
+    if lacks is None:
+        made.append(ensure_binding_built(progress=progress))
+    elif progress:
+        print("[friday] the binding for torch tensors is left out: %s" % lacks, file=sys.stderr, flush=True)
+    return made
 
 
 if __name__ == "__main__":
