@@ -10,9 +10,10 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <stdexcept>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -187,8 +188,8 @@ PyObject* guarded(const char* what, F body) {
     } catch (const Refused& r) {
         PyErr_SetString(refusal, (std::string(what) + ": " + r.why).c_str());
         return nullptr;
-    } catch (const std::exception& e) {      // torch's own: out of memory and the like
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {                          // torch's own, as the exception that torch raises for it (OutOfMemoryError and the like)
+        torch::translate_exception_to_python(std::current_exception());
         return nullptr;
     }
 }

@@ -1,5 +1,5 @@
-"""Kernels whose bounded waits gave up, on streams of the caller's: who is told.  The failures are made on the host: a code is copied to
-where a kernel would leave it, no kernel is made to wait."""
+"""Failures of the operators of a shared prefix: who is told, and as what.  Kernels whose bounded waits gave up: the failure is made on the
+host, a code is copied to where a kernel would leave it, no kernel is made to wait."""
 import ctypes
 
 import numpy as np
@@ -113,3 +113,18 @@ def test_more_streams_than_words():
         assert again.value == words[7]
     finally:
         native.lib().friday_ops_free(handle)
+
+
+def test_no_memory_for_a_result_is_torchs_own_error():
+    x = torch.zeros((1 << 16, 256), device=DEV)
+    pos, denom = torch.zeros((1 << 16, 1), dtype=torch.int32, device=DEV), torch.ones(64, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    room = (torch.cuda.memory_reserved(0) + (8 << 20)) / torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction(room)      # (of this process alone)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            ops.rotate_axes(x, pos, denom, [64], 2, 128)          # a result of 64 MB
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert ops.rotate_axes(x, pos, denom, [64], 2, 128).shape == x.shape
