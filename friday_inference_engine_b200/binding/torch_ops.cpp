@@ -244,8 +244,8 @@ PyObject* rope_axes_kv_write(PyObject*, PyObject* const* argv, Py_ssize_t n) {
         if (n > a.next && argv[a.next] == Py_None) out = at::empty({rows, (int64_t)nq * hd}, qkv.options());
         else out = a.rows("q_out");
         if (out.scalar_type() != qkv.scalar_type()) throw Refused{"qkv and q_out are of one type, got " + text_of(qkv) + " and " + text_of(out)};
-        if (rows > 0 && c.seqs > 0) {
-            if (c.width == 0) throw Refused{"the block table is empty"};
+        if (rows > 0) {
+            if (c.seqs == 0 || c.width == 0) throw Refused{"the block table is empty"};
             void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)a.device).stream();
             int rc;
             Py_BEGIN_ALLOW_THREADS

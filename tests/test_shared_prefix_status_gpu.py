@@ -128,3 +128,14 @@ def test_no_memory_for_a_result_is_torchs_own_error():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert ops.rotate_axes(x, pos, denom, [64], 2, 128).shape == x.shape
+
+
+@pytest.mark.parametrize("shape", [(0, 3), (0, 0), (2, 0)])
+def test_an_append_without_a_table_is_refused(shape):
+    """(It used to hand back queries that nothing had written.)"""
+    qkv, pos = torch.ones((2, 3 * 16), device=DEV), torch.zeros((2, 1), dtype=torch.int32, device=DEV)
+    rows, table = torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(shape, dtype=torch.int32, device=DEV)
+    kp, vp = torch.zeros((1, 64, 1, 16), device=DEV), torch.zeros((1, 64, 1, 16), device=DEV)
+    with pytest.raises(native.KernelError, match="block table is empty"):
+        ops.rope_axes_kv_write(qkv, rows, rows, pos, torch.ones(8, device=DEV), [8], 1, 1, 16, kp, vp, table, 64)
+    assert ops.rope_axes_kv_write(qkv[:0], rows[:0], rows[:0], pos[:0], torch.ones(8, device=DEV), [8], 1, 1, 16, kp, vp, table, 64).shape == (0, 16)
