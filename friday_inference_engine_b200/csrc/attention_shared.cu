@@ -644,23 +644,23 @@ int launch_rows(const SharedArgs& p, int tile_rows, long long ctas, cudaStream_t
 //               numbers a weight) over its scores.  The reference maximum only moves when the true one has grown by more than 8 (in
 //               log2 units; weights stay below 2^8); O is rescaled then.
 //
-// A CTA takes 101 KB of shared memory and half the tensor memory, so two share an SM and one's softmax runs beside the other's
-// products: 16 prompts of 2,188 rows in all behind 8,000 keys, 28 heads on 4 of 128, took 250 us this way and 288 with two tiles and
-// blocks of 128 keys in one CTA per SM; 64 one-token rows behind 16,001 keys 52 and 71.  Now 238 us, 0.99 PFLOP/s: 784 cycles a
-// block of an SM, of which the first product's instructions take 8 x 48 (at 64 keys each reads twice as much of Q as of K) and the
-// second's 4 x 64.  (A fourth of the exponentials as polynomials changes nothing; scores fetched at once so that one buffer serves, with
-// half of Q in tensor memory, 276 us; two threads per row 290.  Two groups of warps that take blocks in turn and hand the reference
-// maximum over took 392 us, 96 registers a thread; tiles of few rows on mma.sync, a block of keys per warp, 1.13 us a block of one CTA
-// where this takes 0.68.)
-//
-// Where jobs are more than CTAs, the CTAs stay and take one job of every round, longest first: 64 one-token rows behind 16,001 keys and
-// 1 to 1,000 of their own 37 us, 48.5 with a CTA per job (both with weights of one bf16 number, see below).
-//
 // Scores, sums, weights and results are 32-bit in effect: P enters the second product as two bf16 numbers, the weight rounded over the
 // first half of its scores' columns and what rounding left over the second half, each with the same values.  One number alone was off by
 // as much again as the result's own rounding (norm of the error against 64 bits 0.0023 of the result's, 0.0017 with two), and which
-// precision a caller got went by page size and alignment; the second product takes twice its time for it: on one card 46 us for 41 (64
+// precision a caller got went by page size and alignment.  The second product takes twice its time for it: on one card 46 us for 41 (64
 // one-token rows behind 16,001), 333 for 273 (the prompts).
+//
+// A CTA takes 101 KB of shared memory and half the tensor memory, so two share an SM and one's softmax runs beside the other's products.
+// 16 prompts of 2,188 rows in all behind 8,000 keys, 28 heads on 4 of 128: 289 us, 0.82 PFLOP/s, and 336 in a run of seconds, whose
+// power lowers the clock.  Of an SM's cycles for a block the first product's instructions take 8 x 48 (at 64 keys each reads twice as much
+// of Q as of K) and the second's 2 x 4 x 64: the tensor core is busy for 72 of 100 cycles.
+//
+// What else was tried, with weights of one number, where the prompts took 238 us and 64 one-token rows behind 16,001 keys 37: two tiles
+// and blocks of 128 keys in one CTA per SM (288 for 250, 71 for 52 then); a fourth of the exponentials as polynomials (no change); scores
+// fetched at once so that one buffer serves, with half of Q in tensor memory (276 us); two threads per row (290); two groups of warps that
+// take blocks in turn and hand the reference maximum over (392, 96 registers a thread); tiles of few rows on mma.sync, a block of keys per
+// warp (1.13 us a block of one CTA for 0.68).  Where jobs are more than CTAs, the CTAs stay and take one job of every round, longest first
+// (64 one-token rows 37 us; 48.5 with a CTA per job).
 //
 // A row's result depends on nothing that it does not see.  Weights there are 0, but zero times infinity is not: in blocks that all rows of
 // the CTA see alike, values of positions that none sees are zeroed in shared memory before the product; in blocks where rows see different
@@ -1246,8 +1246,12 @@ Plan plan_rows(long long rows, int nq, int max_kv_len, int window) {
     return plan;
 }
 
-// What a tile is for a call: its rows and the keys of a block, how many CTAs an SM takes, and what they cost (us; measured): a CTA's
-// begin and end, a block of a full tile beside others (an SM's time over its CTAs) and alone, and one of the rows that a sequence has.
+// What a tile is for a call: its rows and the keys of a block, how many CTAs an SM takes, and what they cost (us; measured with one-token
+// rows of 28 heads of 128, in bf16 with weights of one number): a CTA's begin and end, a block of a full tile beside others (an SM's time
+// over its CTAs) and alone, and one of the rows that a sequence has.  Costs of bf16 do not go by the head size, and weights of two numbers
+// add some 0.1 us to a block: what counts is which way comes out shortest, and in a sweep of forced ways over 13 bf16 shapes the choice was
+// within a tenth of the best one (26.0 us for 23.8 at the worst: 8 x 20 rows behind 2,000).  float32 prompts are further off: 16 x 24 rows
+// of 28 heads behind 1,000 keys are walked whole in 312 us where three shares of the prefix take 225.
 struct TileKind {
     int rows = 0, keys = 0, at_once = 0;                               // rows 0: no tiles for these sizes
     double begin = 0, block = 0, alone = 0, own_block = 0, own_alone = 0;

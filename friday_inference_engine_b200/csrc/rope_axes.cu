@@ -7,8 +7,10 @@
 //            is what sets this apart from rowwise.cu's rope_kv_write: all tokens of an image share a time position.
 //
 // Angles.  A turn is 2^64: a pair's step per position is kept as a 64-bit fraction of a turn, 2^64 / (2 pi denom), formed in double
-// precision; position times step modulo 2^64 is then exactly the angle's fraction of a turn for every 32-bit position (a float
-// division leaves an error of pos * 2^-24, which at position 10^6 is 0.06 rad).  The upper 32 bits go through sincospif.
+// precision (2 pi, its product with denom and the reciprocal are each rounded to 53 bits).  Position times step modulo 2^64 is exact for
+// every 32-bit position, so what the step is off by is all that grows with the position: the angle is off by about pos / denom * 2^-52 rad,
+// 2^-21 at position 2^31 with denom 1 (a float division leaves pos / denom * 2^-24, which at position 10^6 is 0.06 rad).  The upper 32
+// bits go through sincospif.
 #include <math.h>
 
 #include <atomic>
@@ -255,8 +257,10 @@ __global__ void __launch_bounds__(THREADS) rope_axes_kernel(const RopeArgs p, co
 constexpr int RING_THREADS = 256, RING_BLOCKS = 3, RING_ROWS = 64;
 constexpr int RING_ANGLES = 4;                                     // sines and cosines that a thread makes per group, at most
 constexpr int STAGE_BYTES = 22 * 1024, RING_BYTES = 71 * 1024;     // of a group; of all stages and the tables (three blocks per SM)
-// Bytes of rows: below, the kernel above (28 heads on 4 of 128, bf16, us, above / ring: 64 rows 4.08 / 3.94, 200 rows 4.5 / 4.0, 500 rows
-// 7.3 / 5.0; 32 heads of 80: 64 rows 2.9 / 3.9, 200 rows 3.2 / 4.0, 500 rows 4.9 / 4.1).
+// Bytes of rows: below, the kernel above.  Where the two meet differs by layout, between 0.6 and 2 MB (28 heads on 4 of 128, bf16, us, above /
+// ring: 64 rows 4.08 / 3.94, 200 rows 4.5 / 4.0, 500 rows 7.3 / 5.0; 32 heads of 80: 64 rows 2.9 / 3.9, 200 rows 3.2 / 4.0, 500 rows
+// 4.9 / 4.1): this bound is on the far side, so rows of 9 KB take up to 0.5 us longer than the ring would from 0.6 MB on, and no layout
+// takes the ring where that is the slower way.
 constexpr long long RING_FROM = 2 << 20;
 
 __device__ __forceinline__ void bulk_in(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {

@@ -431,7 +431,11 @@ public:
     // row_seq is negative is not written.  Pages that a table leaves out read as zeros.  A row's result depends on nothing that the
     // row does not see; one that gives a weight to a value that is not finite has no finite number there.  The rows of sequence s are
     // ctx.seq_start[s] and the seq_qlen[s] - 1 after it; ctx.max_kv_len bounds the positions (prefix included) and only shares the work out.
-    // Prefix and own keys are read once for all rows that share them.  prefix_len is the host's: a captured call keeps it.
+    // Keys and values are read once per tile of rows (128 rows of a kv head's heads in bf16 with heads of up to 128 that are a multiple of
+    // 16, pages of 64 and rows on 16-byte boundaries, 16 to 64 in float32 with heads of up to 128 that are a multiple of 4; one kv head
+    // has at most that many heads): for the prefix
+    // a tile is of any sequences' rows, or of one sequence's where many rows of each make that the shorter way.  Any other size reads them
+    // once per row and head.  prefix_len is the host's: a captured call keeps it.
     void attention_shared(const Tensor& q, int64_t q_stride, Tensor& out, const CacheView& view, const int* prefix_table, int prefix_len,
                           const StepContext& ctx, int n_heads, int n_kv_heads, int head_dim, int window, float scale,
                           const Place* place = nullptr);

@@ -1,5 +1,5 @@
-"""The library's operations, callable on torch tensors: what the tests of single kernels
-and the measurements use.  Every function marshals its arguments to the C++ operation of
+"""The library's operations, callable on torch tensors, for programs that keep their own
+tensors and caches, the tests of single kernels and the measurements.  Every function marshals its arguments to the C++ operation of
 the same name (ops/ops.cpp, include/friday/ops.h), which chooses and launches this
 library's own CUDA kernels; nothing is computed here, and there is no CPU path.
 
