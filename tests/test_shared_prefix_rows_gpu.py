@@ -130,3 +130,12 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(dtype, head
         int((~finite & ~spoilt).sum()), int((finite & spoilt).sum()))
     b.v_pool = clean                                      # (the definition without them, for all other numbers)
     b.check(torch.where(spoilt, b.reference()[0].to(dtype), out), "numbers beside")
+
+
+# ------------------------------------------------------------------ steps of very unequal sequences
+@pytest.mark.parametrize("dtype,heads,kv_heads,hd,window", [(BF, 28, 4, 128, 0), (BF, 4, 2, 16, 333), (F32, 14, 2, 64, 0)])
+def test_a_long_prompt_beside_one_token_rows(dtype, heads, kv_heads, hd, window):
+    """Most sequences have one row, one has many: most of the jobs that the longest one's tiles give the others have no rows."""
+    q_lens = [1] * 20 + [1501] + [1] * 11
+    b = sp.Batch(dtype, q_lens, [q + 17 * i for i, q in enumerate(q_lens)], 700, heads, kv_heads, hd, window=window, seed=31)
+    b.check(b.run(ops), "a long prompt beside one-token rows")
