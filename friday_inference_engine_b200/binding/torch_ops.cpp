@@ -10,7 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Exceptions.h>
+#include <c10/util/Exception.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
@@ -27,6 +27,7 @@ decltype(&friday_ops_attention_shared) shared_fn = nullptr;
 decltype(&friday_ops_attention_shared_floats) floats_fn = nullptr;
 PyObject* check_code = nullptr;           // native.check
 PyObject* refusal = nullptr;              // native.KernelError
+PyObject* out_of_memory = nullptr;        // torch.OutOfMemoryError
 
 struct Refused {
     std::string why;
@@ -188,8 +189,11 @@ PyObject* guarded(const char* what, F body) {
     } catch (const Refused& r) {
         PyErr_SetString(refusal, (std::string(what) + ": " + r.why).c_str());
         return nullptr;
-    } catch (...) {                          // torch's own, as the exception that torch raises for it (OutOfMemoryError and the like)
-        torch::translate_exception_to_python(std::current_exception());
+    } catch (const c10::OutOfMemoryError& e) {
+        PyErr_SetString(out_of_memory, e.what_without_backtrace());
+        return nullptr;
+    } catch (const std::exception& e) {      // torch's other errors
+        PyErr_SetString(PyExc_RuntimeError, e.what());
         return nullptr;
     }
 }
@@ -314,19 +318,21 @@ PyObject* attention_shared(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     });
 }
 
-// (addresses of the four C functions, native.check, native.KernelError)
+// (addresses of the four C functions, native.check, native.KernelError, torch.OutOfMemoryError)
 PyObject* init(PyObject*, PyObject* args) {
     unsigned long long rotate = 0, append = 0, shared = 0, floats = 0;
-    PyObject *check = nullptr, *error = nullptr;
-    if (!PyArg_ParseTuple(args, "KKKKOO", &rotate, &append, &shared, &floats, &check, &error)) return nullptr;
+    PyObject *check = nullptr, *error = nullptr, *memory = nullptr;
+    if (!PyArg_ParseTuple(args, "KKKKOOO", &rotate, &append, &shared, &floats, &check, &error, &memory)) return nullptr;
     rotate_fn = (decltype(rotate_fn))rotate;
     append_fn = (decltype(append_fn))append;
     shared_fn = (decltype(shared_fn))shared;
     floats_fn = (decltype(floats_fn))floats;
     Py_INCREF(check);
     Py_INCREF(error);
+    Py_INCREF(memory);
     check_code = check;
     refusal = error;
+    out_of_memory = memory;
     Py_RETURN_NONE;
 }
 

@@ -63,7 +63,7 @@ def _torch_ops():
     import importlib.util
     from ctypes import cast
 
-    import torch  # noqa: F401 - its libraries have to be loaded first
+    import torch                         # (its libraries have to be loaded first)
 
     from . import build
     try:
@@ -76,7 +76,7 @@ def _torch_ops():
     library = native.lib()
     module.init(*(cast(getattr(library, "friday_ops_" + name), c_void_p).value
                   for name in ("rotate_axes", "rope_axes_kv_write", "attention_shared", "attention_shared_floats")), native.check,
-                native.KernelError)
+                native.KernelError, torch.OutOfMemoryError)
     _torch_ops = lambda: module          # noqa: E731 - from here on the module itself
     return module
 
