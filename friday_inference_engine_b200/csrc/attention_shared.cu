@@ -1036,16 +1036,17 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             if (mixed(i)) {
                 // Values that are not finite are taken out (zero times infinity is not zero); rows that see them get them at the end.
                 if (!(ok = mbar_wait(v_full + 8 * b, par, p.status, 37))) break;
+                const int key = r & (KEYS - 1);
                 bool found = false;
                 for (int s = 0; s < slices; ++s) {
                     // (a row's eight pieces of 16 bytes shared by two threads, lanes in different banks)
-                    uint32_t* line = (uint32_t*)(s_v + b * STAGE + s * KSLICE + (r & (KEYS - 1)) * 128);
+                    uint32_t* line = (uint32_t*)(s_v + b * STAGE + s * KSLICE + key * 128);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         uint4* const at = (uint4*)line + ((r + (r / KEYS) * 4 + q) & 7);
-                        uint4 v = *at;
+                        const uint4 v = *at;
                         if (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) {
-                            found = true;
+                            found |= key >= in_lo && key <= in_hi;             // (behind the last row's position nobody asks for them)
                             *at = make_uint4(finite_of(v.x), finite_of(v.y), finite_of(v.z), finite_of(v.w));
                         }
                     }
